@@ -232,6 +232,106 @@ int amlike_gmm_score_raw(amlike_gmm_t *gmm, amlike_xform_t *xf, const float *raw
                          int32_t ld, const float *spk_mat, int32_t rows2, int32_t cols2,
                          float log_sum_exp_prune, float *out, int32_t ldo);
 
+/* ---- dense layers in 16 and 8 bits ----------------------------------------- */
+
+/* Operators of residual networks, for models wider than what the components below are used
+ * for: rows = frames (of one stream, of several streams side by side, or of whole utterances
+ * back to back), columns = the layer's width.  They have no counterpart in the reference, whose
+ * NormalizeComponent (nnet2/nnet-component.cc:578-592) and AffineComponent (:1123-1131) they
+ * stand beside (AMLIKE_NORMALIZE, AMLIKE_AFFINE: fp32 in and out).  Forward only.
+ *
+ * None of the *_dev calls allocates, keeps anything from one call for the next or waits for the
+ * GPU: they may be made from several threads and streams at once with one handle, and be
+ * recorded into HIP graphs. */
+
+enum amlike_type {
+  AMLIKE_F32 = 0,
+  AMLIKE_BF16 = 1,
+  AMLIKE_F16 = 2,
+  AMLIKE_MX8 = 3 /* e4m3 values (no infinities, largest 448) with one scale per 32 consecutive columns
+                    of a row: an e8m0 byte, 2^(byte - 127).  Written so: k is the smallest integer
+                    >= -127 with max |finite y of the group| <= 448 * 2^k, the scale byte is k + 127,
+                    a value is y * 2^-k rounded to nearest even; what is not finite becomes NaN.
+                    The last group of a row is short where the columns are no multiple of 32. */
+};
+
+/* Where a matrix lies in device memory.  Element (r, c) of a 16- or 32-bit matrix is
+ * data[r * ld + c]; data is aligned to its element.  AMLIKE_MX8: data are bytes, and the scale
+ * of (r, c) is scales[r * ld_scales + c / 32].  Any ld >= the columns, any ld_scales >=
+ * ceil(columns / 32); what lies behind a row's columns and behind the last row is neither
+ * needed nor written.  Rows that start on 16 bytes (and MX8 scales on 4) are the fast case. */
+typedef struct amlike_matrix {
+  void *data;
+  void *scales; /* AMLIKE_MX8 only, else NULL */
+  int64_t ld;        /* elements */
+  int64_t ld_scales; /* bytes; AMLIKE_MX8 only */
+  int32_t type;      /* enum amlike_type */
+} amlike_matrix_t;
+
+/* y[r][c] = x[r][c] in out's type (rounded to nearest even; 16-bit overflow gives infinities).
+ * x: F32, BF16 or F16; out: any type.  rows may be 0.  Runs on the device of the calling thread
+ * (amlike_init) and on `stream`.  x and out must not overlap. */
+int amlike_convert_dev(const amlike_matrix_t *x, int32_t rows, int32_t cols, const amlike_matrix_t *out,
+                       void *stream);
+
+typedef struct amlike_norm amlike_norm_t;
+
+/* s = x + residual (residual == NULL: s = x);  out = s / sqrt(mean over the row of s^2 + eps) * weight.
+ * weight: [dim] host array or NULL (ones); 1 <= dim <= 32768; 1e-30 <= eps <= 1.
+ * s is held in fp32: the mean and out come from the unrounded s, which is stored rounded to the
+ * type of `sum`.  A row that holds a NaN gives a row of NaNs, one that holds an infinity NaN there and zeros
+ * elsewhere, as the formula does. */
+int amlike_norm_create(const float *weight, int32_t dim, float eps, amlike_norm_t **out);
+int amlike_norm_destroy(amlike_norm_t *norm);
+int32_t amlike_norm_dim(const amlike_norm_t *norm);
+int32_t amlike_norm_device(const amlike_norm_t *norm);
+/* Device pointers, asynchronous.  x: F32, BF16 or F16; residual (or NULL) and sum (or NULL: not
+ * stored) have x's type; out: any type.  rows may be 0.  sum and out may each be the same matrix
+ * (same data, type and ld) as x or residual; no other overlap is allowed. */
+int amlike_norm_apply_dev(const amlike_norm_t *norm, const amlike_matrix_t *x,
+                          const amlike_matrix_t *residual, int32_t rows, const amlike_matrix_t *sum,
+                          const amlike_matrix_t *out, void *stream);
+/* Host pointers, fp32, synchronous; residual and sum may be NULL (sum needs no residual). */
+int amlike_norm_apply(amlike_norm_t *norm, const float *x, int32_t ld, const float *residual, int32_t ldr,
+                      int32_t rows, float *sum, int32_t lds, float *out, int32_t ldo);
+
+enum amlike_activation {
+  AMLIKE_ACT_NONE = 0,
+  AMLIKE_ACT_RELU = 1,
+  AMLIKE_ACT_SIGMOID = 2,
+  AMLIKE_ACT_TANH = 3,
+  AMLIKE_ACT_SILU = 4, /* x / (1 + exp(-x)) */
+  AMLIKE_ACT_GELU = 5  /* x (1 + erf(x / sqrt 2)) / 2 */
+};
+
+typedef struct amlike_linear amlike_linear_t;
+
+/* out = act(x weights^T + bias) + residual, products of `type` (BF16, F16 or MX8) summed in fp32.
+ * weights: [output_dim x input_dim] host array with row stride ld, rounded once to `type` (MX8:
+ * groups of 32 along a row as above); bias: [output_dim] host array or NULL, kept in fp32.
+ * Both dimensions up to 2^20.  AMLIKE_ENONFINITE when a weight is not finite in `type` or a bias
+ * is not finite. */
+int amlike_linear_create(const float *weights, int32_t ld, const float *bias, int32_t input_dim,
+                         int32_t output_dim, int32_t type, amlike_linear_t **out);
+int amlike_linear_destroy(amlike_linear_t *linear);
+int32_t amlike_linear_input_dim(const amlike_linear_t *linear);
+int32_t amlike_linear_output_dim(const amlike_linear_t *linear);
+int32_t amlike_linear_type(const amlike_linear_t *linear);
+int32_t amlike_linear_device(const amlike_linear_t *linear);
+/* Device pointers, asynchronous.  x [rows x input_dim] has the handle's type; residual (F32, BF16
+ * or F16, or NULL) and out (any type) are [rows x output_dim].  rows may be 0.  out may be the
+ * same matrix as residual (same data, type and ld); no other overlap is allowed.  A row's result
+ * does not depend on the other rows' values.  MX8 layers: for an F32 output the products are
+ * summed as exactly as those of the other types; for the smaller outputs by the 8-bit matrix
+ * instruction, whose sums are about 1.5e-5 off, relative to the sum of normal values, and twice
+ * as fast. */
+int amlike_linear_apply_dev(const amlike_linear_t *linear, const amlike_matrix_t *x, int32_t rows,
+                            int32_t activation, const amlike_matrix_t *residual,
+                            const amlike_matrix_t *out, void *stream);
+/* Host pointers, fp32, synchronous: x is converted to the handle's type on the device. */
+int amlike_linear_apply(amlike_linear_t *linear, const float *x, int32_t ld, int32_t rows,
+                        int32_t activation, const float *residual, int32_t ldr, float *out, int32_t ldo);
+
 /* ---- nnet2 forward -------------------------------------------------------- */
 
 /* Component kinds of the nnet2 forward path

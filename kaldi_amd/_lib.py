@@ -5,7 +5,7 @@ There is no fallback: if the shared object is missing, loading raises.
 """
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int32, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # AMLIKE_LIB_PATH: another build of the same library (tuning aid for A/B runs)
@@ -32,8 +32,14 @@ class Component(ctypes.Structure):
     ]
 
 
+class Matrix(ctypes.Structure):
+    """struct amlike_matrix of include/amlike.h."""
+    _fields_ = [("data", c_void_p), ("scales", c_void_p), ("ld", c_int64), ("ld_scales", c_int64), ("type", c_int32)]
+
+
 def _declare(lib):
     fp, ip = POINTER(c_float), POINTER(c_int32)
+    mp = POINTER(Matrix)
     sigs = {
         "amlike_init": (ctypes.c_int, [ctypes.c_int]),
         "amlike_last_error": (c_char_p, []),
@@ -72,6 +78,21 @@ def _declare(lib):
         "amlike_gmm_profile_kernel": (ctypes.c_int, [c_void_p, c_int32]),
         "amlike_gmm_kernel_time": (ctypes.c_int, [c_void_p, POINTER(c_float), ip]),
         "amlike_gmm_time_score_dev": (ctypes.c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_int32, POINTER(c_float)]),
+        "amlike_convert_dev": (ctypes.c_int, [mp, c_int32, c_int32, mp, c_void_p]),
+        "amlike_norm_create": (ctypes.c_int, [fp, c_int32, c_float, POINTER(c_void_p)]),
+        "amlike_norm_destroy": (ctypes.c_int, [c_void_p]),
+        "amlike_norm_dim": (c_int32, [c_void_p]),
+        "amlike_norm_device": (c_int32, [c_void_p]),
+        "amlike_norm_apply_dev": (ctypes.c_int, [c_void_p, mp, mp, c_int32, mp, mp, c_void_p]),
+        "amlike_norm_apply": (ctypes.c_int, [c_void_p, fp, c_int32, fp, c_int32, c_int32, fp, c_int32, fp, c_int32]),
+        "amlike_linear_create": (ctypes.c_int, [fp, c_int32, fp, c_int32, c_int32, c_int32, POINTER(c_void_p)]),
+        "amlike_linear_destroy": (ctypes.c_int, [c_void_p]),
+        "amlike_linear_input_dim": (c_int32, [c_void_p]),
+        "amlike_linear_output_dim": (c_int32, [c_void_p]),
+        "amlike_linear_type": (c_int32, [c_void_p]),
+        "amlike_linear_device": (c_int32, [c_void_p]),
+        "amlike_linear_apply_dev": (ctypes.c_int, [c_void_p, mp, c_int32, c_int32, mp, mp, c_void_p]),
+        "amlike_linear_apply": (ctypes.c_int, [c_void_p, fp, c_int32, c_int32, c_int32, fp, c_int32, fp, c_int32]),
         "amlike_nnet_create": (ctypes.c_int, [POINTER(Component), c_int32, fp, c_int32, POINTER(c_void_p)]),
         "amlike_nnet_destroy": (ctypes.c_int, [c_void_p]),
         "amlike_nnet_input_dim": (c_int32, [c_void_p]),

@@ -1,0 +1,632 @@
+// out = act(x W^T + b) + r: a matrix product of 16-bit or 8-bit operands on the matrix
+// instructions, summed in fp32, with the bias, the activation and the residual in its epilogue
+// (amlike_linear_*).
+//
+// Layout.  A k-tile is 128 bytes of a row: 64 columns in 16 bits, 128 in 8.  Both kinds of matrix
+// instruction used (16x16x32 bf16 / f16, 16x16x128 scaled e4m3) then look alike: lane l of a
+// fragment holds row l % 16 and, of its k-tile, the 32 bytes l / 16 -- the 16-bit ones as two
+// instructions of 16 bytes each (which columns meet in one instruction does not matter as long as
+// both operands agree), the 8-bit one as a single instruction whose scale is that lane's byte.
+// W is the instructions' first operand and x the second, so that a lane's results are 4
+// consecutive outputs of one row of x per fragment; rows of W are stored in an order (PhysicalRow)
+// that makes them 16 consecutive outputs over four fragments.
+// The 8-bit instruction aligns the products of a few neighbouring columns to the largest of them
+// and drops what lies more than 13 binary places below it (measured: 2^16 + 2^2 is 2^16, 2^16 + 2^3
+// is whole), which leaves a relative error of about 1.5e-5 in a sum of normal values whatever its
+// length: far below the rounding of a 16-bit (2^-9, 2^-12 on average) or 8-bit output, too much for
+// an fp32 one.  For an fp32 output the 8-bit operands are therefore widened to bf16, which holds
+// value times scale exactly, and multiplied there (kMx8Exact), at half the matrix rate.
+//   W:      [k-tile][row, physical order, padded to 64][128 bytes], zeros behind both ends
+//   scales: [k-tile][row, the same order][4 bytes], 2^0 behind both ends  (8 bits only)
+#include <algorithm>
+#include <mutex>
+#include <new>
+
+#include "dense_common.h"
+
+namespace amlike {
+
+constexpr int kTileBytes = 128;  // of a row in a k-tile
+constexpr int kChunks = 8;       // 16-byte pieces of it
+constexpr int kLinearMaxDim = 1 << 20;   // either dimension of a layer
+
+// Within 64 outputs: where output n = g * 16 + f * 4 + i is stored: row f * 16 + g * 4 + i, row
+// g * 4 + i of fragment f.  The map is its own inverse.
+__host__ __device__ constexpr int PhysicalRow(int n) { return (n & ~63) | (n & 3) | (n >> 2 & 12) | (n << 2 & 48); }
+
+struct LinearArgs {
+  const uint8_t *x, *x_scales;  // [rows][k], row strides in bytes
+  const uint8_t *w;
+  const uint32_t *w_scales;
+  const float *bias;  // [n padded to 64]
+  const void *res;
+  void *out;
+  uint8_t *out_scales;
+  int64_t ldx, ld_xs, ldr, ldo, ld_os;
+  int32_t rows, k, n, n_pad, k_tiles;
+  int32_t act, res_type, out_type;  // res_type -1: none
+};
+
+// The kernels' kinds of product: a layer's type, or 8-bit operands with bf16 products.
+constexpr int kMx8Exact = 4;
+__host__ __device__ constexpr bool IsMx8(int kind) { return kind == AMLIKE_MX8 || kind == kMx8Exact; }
+
+template <int TYPE>
+struct Frag;
+template <>
+struct Frag<AMLIKE_BF16> {
+  typedef __bf16 vec __attribute__((ext_vector_type(8)));
+};
+template <>
+struct Frag<AMLIKE_F16> {
+  typedef _Float16 vec __attribute__((ext_vector_type(8)));
+};
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// A 16-byte piece of e4m3 values times their scale (an e8m0 byte), as two fragments of bf16.
+__device__ __forceinline__ void widen(const u32x4 p, uint32_t scale_byte, Frag<AMLIKE_BF16>::vec out[2]) {
+  // (2^-127 is a denormal: the byte's bits in an exponent field would be 0)
+  const float s = as_float(scale_byte ? scale_byte << 23 : 0x400000u);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const f32x2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)p[q], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)p[q], true);
+    out[q >> 1][(q & 1) * 4 + 0] = (__bf16)(a[0] * s);
+    out[q >> 1][(q & 1) * 4 + 1] = (__bf16)(a[1] * s);
+    out[q >> 1][(q & 1) * 4 + 2] = (__bf16)(b[0] * s);
+    out[q >> 1][(q & 1) * 4 + 3] = (__bf16)(b[1] * s);
+  }
+}
+
+// What a lane feeds the matrix instructions from pieces g and g + 4 of a row in one k-tile, and the
+// word of the row's four scales.
+template <int KIND>
+struct Operand {
+  u32x4 p[2];
+  int scale;
+  __device__ __forceinline__ void set(u32x4 p0, u32x4 p1, uint32_t scales, int g) {
+    p[0] = p0;
+    p[1] = p1;
+    scale = (int)(scales >> (8 * g));  // the instruction takes the lowest byte
+  }
+};
+template <>
+struct Operand<kMx8Exact> {
+  Frag<AMLIKE_BF16>::vec v[4];
+  __device__ __forceinline__ void set(u32x4 p0, u32x4 p1, uint32_t scales, int g) {
+    widen(p0, scales >> (8 * (g >> 1)) & 0xff, v);  // piece c holds columns of group c / 2
+    widen(p1, scales >> (16 + 8 * (g >> 1)) & 0xff, v + 2);
+  }
+};
+
+// One k-tile of a fragment of W and one of x: c += W x^T.
+template <int TYPE>
+__device__ __forceinline__ f32x4v tile_product(const Operand<TYPE> &ow, const Operand<TYPE> &ox, f32x4v c) {
+  if constexpr (TYPE == kMx8Exact) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ow.v[h], ox.v[h], c, 0, 0, 0);
+    return c;
+  } else if constexpr (TYPE == AMLIKE_MX8) {
+    const u32x4 *w = ow.p, *x = ox.p;
+    const i32x8 a = {(int)w[0][0], (int)w[0][1], (int)w[0][2], (int)w[0][3], (int)w[1][0], (int)w[1][1], (int)w[1][2], (int)w[1][3]};
+    const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, ow.scale, 0, ox.scale);
+  } else {
+    typedef typename Frag<TYPE>::vec V;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const V a = __builtin_bit_cast(V, ow.p[h]), b = __builtin_bit_cast(V, ox.p[h]);
+      if constexpr (TYPE == AMLIKE_BF16) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+      else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    return c;
+  }
+}
+
+// ---- epilogue ----------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+
+// Phi(-a), a >= 0: exp(-a^2/2) times erfcx(a / sqrt 2) / 2, the latter as a polynomial in
+// t = 1 / (1 + p a) fitted by least squares iterated towards the smallest largest relative error
+// on [0, 14] (beyond, the exponential is 0).  Degree 8 without constant: 1.5e-7 off, for fp32
+// outputs; degree 5: 3.5e-5, less than a tenth of the rounding to f16 (4.9e-4).
+template <bool EXACT>
+__device__ __forceinline__ float normal_tail(float a) {
+  const float e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170368f);
+  float t, p;
+  if constexpr (EXACT) {
+    t = __builtin_amdgcn_rcpf(fmaf(0.30f, a, 1.0f));
+    p = 0.0356770197f;
+    p = fmaf(p, t, -0.157212402f);
+    p = fmaf(p, t, 0.206369481f);
+    p = fmaf(p, t, -0.0536982531f);
+    p = fmaf(p, t, 0.128569295f);
+    p = fmaf(p, t, 0.0999111902f);
+    p = fmaf(p, t, 0.120754321f);
+    p = fmaf(p, t, 0.119629275f);
+  } else {
+    t = __builtin_amdgcn_rcpf(fmaf(0.38f, a, 1.0f));
+    p = -0.0899287643f;
+    p = fmaf(p, t, 0.188877211f);
+    p = fmaf(p, t, 0.0919794799f);
+    p = fmaf(p, t, 0.157829353f);
+    p = fmaf(p, t, 0.151225193f);
+  }
+  return p * t * e;
+}
+
+// tanh: near 0, where 1 - 2 / (1 + exp(2x)) cancels, x times an even polynomial (fitted as above
+// on [0, .65], 1.5e-7 off).
+__device__ __forceinline__ float fast_tanh(float x) {
+  const float a = __builtin_fabsf(x), z = x * x;
+  float p = 0.0146252109f;
+  p = fmaf(p, z, -0.0515180279f);
+  p = fmaf(p, z, 0.132978768f);
+  p = fmaf(p, z, -0.333315005f);
+  p = fmaf(p, z, 0.999999846f);
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp(2.0f * a));
+  return a < 0.6f ? x * p : __builtin_copysignf(far, x);
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-x)); }
+
+template <int N>
+__device__ __forceinline__ void activate(int act, bool exact, float *v) {
+  if (act == AMLIKE_ACT_NONE) return;
+  if (act == AMLIKE_ACT_RELU) {  // (a comparison: NaN stays)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+  } else if (act == AMLIKE_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = sigmoid(v[i]);
+  } else if (act == AMLIKE_ACT_TANH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = fast_tanh(v[i]);
+  } else if (act == AMLIKE_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
+  } else if (exact) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float q = normal_tail<true>(__builtin_fabsf(v[i]));
+      v[i] *= v[i] > 0.0f ? 1.0f - q : q;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float q = normal_tail<false>(__builtin_fabsf(v[i]));
+      v[i] *= v[i] > 0.0f ? 1.0f - q : q;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t quad_max_bits(uint32_t u) {
+  u = max(u, (uint32_t)__builtin_amdgcn_mov_dpp((int)u, 0xB1, 0xF, 0xF, true));
+  return max(u, (uint32_t)__builtin_amdgcn_mov_dpp((int)u, 0x4E, 0xF, 0xF, true));
+}
+
+// Sums of eight consecutive outputs n .. n + 7 (n a multiple of 8) of row m become output; four
+// neighbouring lanes hold a group of 32.  Every lane of a quad calls it, m >= rows or n >= n's end
+// included.
+__device__ __forceinline__ void finish8(const LinearArgs &a, int64_t m, int n, float v[8]) {
+  const int cols = m < a.rows ? a.n - n : 0;
+  if (cols > 0) {
+    const f32x4v b0 = *reinterpret_cast<const f32x4v *>(a.bias + n), b1 = *reinterpret_cast<const f32x4v *>(a.bias + n + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] += b0[i];
+      v[4 + i] += b1[i];
+    }
+    activate<8>(a.act, a.out_type == AMLIKE_F32, v);
+    if (a.res_type >= 0) {
+      float r[8];
+      load8_any(a.res_type, a.res, m * a.ldr + n, cols, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += r[i];
+    }
+  }
+  if (a.out_type == AMLIKE_MX8) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, i < cols ? finite_bits(v[i]) : 0u);
+    const int k = mx8_exponent(quad_max_bits(top));
+    if (cols > 0) {
+      const u32x2 w = {mx8_pack4(v, k), mx8_pack4(v + 4, k)};
+      store8_bytes(static_cast<uint8_t *>(a.out), m * a.ldo + n, cols, w);
+      if ((n & 31) == 0) a.out_scales[m * a.ld_os + (n >> 5)] = (uint8_t)(k + 127);
+    }
+  } else if (cols > 0) {
+    store8_any(a.out_type, a.out, m * a.ldo + n, cols, v);
+  }
+}
+
+// ---- operands ----------------------------------------------------------------------------------------
+
+// Bytes [at, at + 16) of a row of x as columns, those at the row's end `bytes` and beyond as 0.
+__device__ __forceinline__ u32x4 load_chunk(const uint8_t *row, int at, int bytes) {
+  typedef u32x4 u32x4_byte __attribute__((aligned(1)));
+  u32x4 q = {0, 0, 0, 0};
+  if (at + 16 <= bytes) {
+    q = *reinterpret_cast<const u32x4_byte *>(row + at);
+  } else if (at < bytes) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (at + i < bytes) q[i >> 2] |= (uint32_t)row[at + i] << (8 * (i & 3));
+  }
+  return q;
+}
+// The four scale bytes of k-tile kt of a row of x; 2^0 behind the last group.
+__device__ __forceinline__ uint32_t load_scales(const uint8_t *row, int kt, int groups) {
+  uint32_t s = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s |= (kt * 4 + i < groups ? (uint32_t)row[kt * 4 + i] : 127u) << (8 * i);
+  return s;
+}
+
+// Where 16-byte piece c of row r of a tile lies in LDS: pieces of neighbouring rows are turned
+// against each other, so that 16 lanes reading the same piece of 16 rows meet all banks.
+__device__ __forceinline__ int lds_piece(int r, int c) { return r * kChunks + (c ^ (r >> 1 & 7)); }
+
+// ---- the plain tile kernel: any size, alignment and type ----------------------------------------------
+// 64 x 64 outputs per block of four waves (32 x 32 each); k-tiles go through registers into LDS.
+template <int TYPE>
+__global__ __launch_bounds__(256) void linear_tile_kernel(LinearArgs a) {
+  __shared__ u32x4 s_w[64 * kChunks], s_x[64 * kChunks];
+  __shared__ uint32_t s_ws[64], s_xs[64];
+  __shared__ float s_c[64][68];
+  constexpr bool kMx = IsMx8(TYPE);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wn = (wave & 1) * 32, wm = (wave >> 1) * 32, r16 = lane & 15, g = lane >> 4;
+  const int n_tiles = a.n_pad >> 6;
+  const int n0 = (int)(blockIdx.x % n_tiles) * 64;
+  const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * 64;
+  const int bytes = a.k * (kMx ? 1 : 2), groups = (a.k + 31) >> 5;
+  f32x4v acc[2][2] = {};
+  for (int kt = 0; kt < a.k_tiles; ++kt) {
+    u32x4 qw[2], qx[2];
+    uint32_t sc = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = tid + i * 256, r = p >> 3, c = p & 7;
+      qw[i] = *reinterpret_cast<const u32x4 *>(a.w + ((int64_t)kt * a.n_pad + n0 + r) * kTileBytes + c * 16);
+      const int64_t m = min(m0 + r, (int64_t)a.rows - 1);
+      qx[i] = load_chunk(a.x + m * a.ldx, kt * kTileBytes + c * 16, bytes);
+    }
+    if constexpr (kMx) {
+      if (tid < 64) sc = a.w_scales[(int64_t)kt * a.n_pad + n0 + tid];
+      else if (tid < 128) sc = load_scales(a.x_scales + min(m0 + tid - 64, (int64_t)a.rows - 1) * a.ld_xs, kt, groups);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = tid + i * 256, r = p >> 3, c = p & 7;
+      s_w[lds_piece(r, c)] = qw[i];
+      s_x[lds_piece(r, c)] = qx[i];
+    }
+    if constexpr (kMx) {
+      if (tid < 64) s_ws[tid] = sc;
+      else if (tid < 128) s_xs[tid - 64] = sc;
+    }
+    __syncthreads();
+    Operand<TYPE> fw[2], fx[2];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const int rw = wn + f * 16 + r16, rx = wm + f * 16 + r16;
+      fw[f].set(s_w[lds_piece(rw, g)], s_w[lds_piece(rw, g + 4)], kMx ? s_ws[rw] : 0, g);
+      fx[f].set(s_x[lds_piece(rx, g)], s_x[lds_piece(rx, g + 4)], kMx ? s_xs[rx] : 0, g);
+    }
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc[f][e] = tile_product<TYPE>(fw[f], fx[e], acc[f][e]);
+  }
+  // lane (r16, g): row r16 of fragment e of x; of fragment wn / 16 + f of W outputs g * 16 + that * 4 ..
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<f32x4v *>(&s_c[wm + e * 16 + r16][g * 16 + (wn / 16 + f) * 4]) = acc[f][e];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int p = tid + i * 256, m = p >> 3, c = p & 7;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = s_c[m][c * 8 + j];
+    finish8(a, m0 + m, n0 + c * 8, v);
+  }
+}
+
+// ---- packing the weights ---------------------------------------------------------------------------------
+
+// One 16-byte piece of the packed W per thread, from rows already in the handle's type.
+__global__ __launch_bounds__(256) void linear_pack_kernel(const uint8_t *__restrict__ src, int type, int n, int k,
+                                                          int n_pad, int64_t pieces, u32x4 *__restrict__ dst,
+                                                          int *__restrict__ bad) {
+  for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < pieces; p += (int64_t)gridDim.x * 256) {
+    const int c = (int)(p & 7);
+    const int64_t tr = p >> 3;
+    const int kt = (int)(tr / n_pad), row = PhysicalRow((int)(tr - (int64_t)kt * n_pad));
+    const int es = type == AMLIKE_MX8 ? 1 : 2;
+    u32x4 q = {0, 0, 0, 0};
+    if (row < n) q = load_chunk(src + (int64_t)row * k * es, kt * kTileBytes + c * 16, k * es);
+    dst[p] = q;
+    bool no = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (type == AMLIKE_MX8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) no |= (q[i] >> (8 * j) & 0x7f) == 0x7f;
+      } else {
+        const uint32_t e = type == AMLIKE_BF16 ? 0x7f80u : 0x7c00u;
+        no |= (q[i] & e) == e || (q[i] >> 16 & e) == e;
+      }
+    }
+    if (no) ctl_or(bad, 1);
+  }
+}
+__global__ __launch_bounds__(256) void linear_pack_scales_kernel(const uint8_t *__restrict__ src, int n, int k, int n_pad,
+                                                                 int64_t words, uint32_t *__restrict__ dst) {
+  const int groups = (k + 31) >> 5;
+  for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < words; p += (int64_t)gridDim.x * 256) {
+    const int kt = (int)(p / n_pad), row = PhysicalRow((int)(p - (int64_t)kt * n_pad));
+    dst[p] = row < n ? load_scales(src + (int64_t)row * groups, kt, groups) : 0x7f7f7f7fu;
+  }
+}
+
+}  // namespace amlike
+
+using namespace amlike;
+
+struct amlike_linear {
+  int device = 0;
+  int k = 0, n = 0, n_pad = 0, k_tiles = 0, type = 0;
+  uint8_t *d_w = nullptr;
+  uint32_t *d_scales = nullptr;
+  float *d_bias = nullptr;
+  // the host-pointer call's own stream and buffers
+  hipStream_t stream = nullptr;
+  DeviceBuffer ws_x, ws_q, ws_r, ws_out;
+  std::mutex mu;
+};
+
+namespace amlike {
+namespace {
+
+int PackWeights(amlike_linear *h, const float *weights, int64_t ld, const float *bias) {
+  const size_t row = (size_t)h->k * sizeof(float);
+  const int es = TypeBytes(h->type), groups = (h->k + 31) / 32;
+  const int64_t pieces = (int64_t)h->k_tiles * h->n_pad * kChunks;
+  DeviceBuffer src, typed, scales, flag;
+  auto work = [&]() -> int {
+    int rc = src.Reserve(row * h->n);
+    if (rc == AMLIKE_OK) rc = typed.Reserve((size_t)h->n * h->k * es);
+    if (rc == AMLIKE_OK && h->type == AMLIKE_MX8) rc = scales.Reserve((size_t)h->n * groups);
+    if (rc == AMLIKE_OK) rc = flag.Reserve(sizeof(int));
+    if (rc != AMLIKE_OK) return rc;
+    AMLIKE_HIP(hipMalloc(reinterpret_cast<void **>(&h->d_w), (size_t)pieces * 16));
+    AMLIKE_HIP(hipMalloc(reinterpret_cast<void **>(&h->d_bias), (size_t)h->n_pad * sizeof(float)));
+    rc = ClearWords(static_cast<int *>(flag.ptr), 1, h->stream);
+    if (rc == AMLIKE_OK) rc = ClearWords(reinterpret_cast<int *>(h->d_bias), h->n_pad, h->stream);
+    if (rc != AMLIKE_OK) return rc;
+    if (bias) AMLIKE_HIP(hipMemcpyAsync(h->d_bias, bias, (size_t)h->n * sizeof(float), hipMemcpyHostToDevice, h->stream));
+    AMLIKE_HIP(hipMemcpy2DAsync(src.ptr, row, weights, (size_t)ld * sizeof(float), row, h->n, hipMemcpyHostToDevice, h->stream));
+    const amlike_matrix_t ms = {src.ptr, nullptr, h->k, 0, AMLIKE_F32}, mt = {typed.ptr, scales.ptr, h->k, groups, h->type};
+    rc = LaunchConvert(ms, h->n, h->k, mt, h->stream);
+    if (rc != AMLIKE_OK) return rc;
+    hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 16)), dim3(256), 0,
+                       h->stream, static_cast<const uint8_t *>(typed.ptr), h->type, h->n, h->k, h->n_pad, pieces,
+                       reinterpret_cast<u32x4 *>(h->d_w), static_cast<int *>(flag.ptr));
+    AMLIKE_HIP(hipGetLastError());
+    if (h->type == AMLIKE_MX8) {
+      const int64_t words = (int64_t)h->k_tiles * h->n_pad;
+      AMLIKE_HIP(hipMalloc(reinterpret_cast<void **>(&h->d_scales), (size_t)words * 4));
+      hipLaunchKernelGGL(linear_pack_scales_kernel, dim3((unsigned)std::min<int64_t>((words + 255) / 256, 1 << 16)), dim3(256), 0,
+                         h->stream, static_cast<const uint8_t *>(scales.ptr), h->n, h->k, h->n_pad, words, h->d_scales);
+      AMLIKE_HIP(hipGetLastError());
+    }
+    int bad = 0;
+    AMLIKE_HIP(hipMemcpyAsync(&bad, flag.ptr, sizeof(int), hipMemcpyDeviceToHost, h->stream));
+    AMLIKE_HIP(hipStreamSynchronize(h->stream));
+    if (bad) {
+      SetError("amlike_linear_create: a weight is not finite in the layer's type");
+      return AMLIKE_ENONFINITE;
+    }
+    return AMLIKE_OK;
+  };
+  const int rc = work();
+  if (rc != AMLIKE_OK) (void)hipStreamSynchronize(h->stream);
+  src.Free();
+  typed.Free();
+  scales.Free();
+  flag.Free();
+  return rc;
+}
+
+// Calls `launch` on stretches of the rows, all of them but for outputs beyond 2^35 elements: a grid
+// holds less than 2^32 threads, 2^24 blocks of 256.
+template <typename F>
+int ByRows(LinearArgs a, F launch) {
+  const int64_t most = std::max<int64_t>(((int64_t)1 << 35) / a.n_pad / 256 * 256, 256);
+  const int64_t rows = a.rows;
+  const int rb = a.res_type < 0 ? 0 : TypeBytes(a.res_type), ob = TypeBytes(a.out_type);
+  for (int64_t r = 0; r < rows; r += most) {
+    a.rows = (int32_t)std::min(most, rows - r);
+    if (int rc = launch(a)) return rc;
+    a.x += most * a.ldx;
+    if (a.x_scales) a.x_scales += most * a.ld_xs;
+    if (a.res) a.res = static_cast<const char *>(a.res) + most * a.ldr * rb;
+    a.out = static_cast<char *>(a.out) + most * a.ldo * ob;
+    if (a.out_scales) a.out_scales += most * a.ld_os;
+  }
+  return AMLIKE_OK;
+}
+
+template <int TYPE>
+int LaunchLinear(const LinearArgs &args, hipStream_t st) {
+  return ByRows(args, [&](const LinearArgs &a) -> int {
+    const int64_t tiles = ((int64_t)a.rows + 63) / 64 * (a.n_pad / 64);
+    hipLaunchKernelGGL(linear_tile_kernel<TYPE>, dim3((unsigned)tiles), dim3(256), 0, st, a);
+    AMLIKE_HIP(hipGetLastError());
+    return AMLIKE_OK;
+  });
+}
+
+}  // namespace
+}  // namespace amlike
+
+extern "C" {
+
+int amlike_linear_create(const float *weights, int32_t ld, const float *bias, int32_t input_dim, int32_t output_dim,
+                         int32_t type, amlike_linear_t **out) {
+  if (int rc = BindThread()) return rc;
+  if (!out || !weights || input_dim <= 0 || output_dim <= 0 || input_dim > kLinearMaxDim || output_dim > kLinearMaxDim ||
+      ld < input_dim || (type != AMLIKE_BF16 && type != AMLIKE_F16 && type != AMLIKE_MX8)) {
+    SetError("amlike_linear_create: invalid argument (dimensions 1 to %d, type BF16, F16 or MX8)", kLinearMaxDim);
+    return AMLIKE_EINVAL;
+  }
+  *out = nullptr;
+  if (bias)
+    for (int i = 0; i < output_dim; ++i)
+      if (!(bias[i] - bias[i] == 0.0f)) {
+        SetError("amlike_linear_create: bias %d is not finite", i);
+        return AMLIKE_ENONFINITE;
+      }
+  if (CurrentDevice() < 0) {
+    if (int rc = amlike_init(0)) return rc;
+  }
+  amlike_linear *h = new (std::nothrow) amlike_linear;
+  if (!h) {
+    SetError("amlike_linear_create: out of host memory");
+    return AMLIKE_EOOM;
+  }
+  h->device = CurrentDevice();
+  h->k = input_dim;
+  h->n = output_dim;
+  h->type = type;
+  h->n_pad = (output_dim + 63) / 64 * 64;
+  h->k_tiles = (int)(((int64_t)input_dim * TypeBytes(type) + kTileBytes - 1) / kTileBytes);
+  const hipError_t e = hipStreamCreateWithFlags(&h->stream, hipStreamNonBlocking);
+  int rc = AMLIKE_OK;
+  if (e != hipSuccess) {
+    SetError("amlike_linear_create: %s", hipGetErrorString(e));
+    rc = AMLIKE_EHIP;
+  }
+  if (rc == AMLIKE_OK) rc = PackWeights(h, weights, ld, bias);
+  if (rc != AMLIKE_OK) {
+    amlike_linear_destroy(h);
+    return rc;
+  }
+  *out = h;
+  return AMLIKE_OK;
+}
+
+int amlike_linear_destroy(amlike_linear_t *h) {
+  if (int rc = BindHandle(h)) return rc;
+  if (!h) return AMLIKE_OK;
+  (void)hipFree(h->d_w);
+  (void)hipFree(h->d_scales);
+  (void)hipFree(h->d_bias);
+  h->ws_x.Free();
+  h->ws_q.Free();
+  h->ws_r.Free();
+  h->ws_out.Free();
+  if (h->stream) (void)hipStreamDestroy(h->stream);
+  delete h;
+  return AMLIKE_OK;
+}
+
+int32_t amlike_linear_input_dim(const amlike_linear_t *h) { return h ? h->k : 0; }
+int32_t amlike_linear_output_dim(const amlike_linear_t *h) { return h ? h->n : 0; }
+int32_t amlike_linear_type(const amlike_linear_t *h) { return h ? h->type : -1; }
+int32_t amlike_linear_device(const amlike_linear_t *h) { return h ? h->device : -1; }
+
+int amlike_linear_apply_dev(const amlike_linear_t *h, const amlike_matrix_t *x, int32_t rows, int32_t activation,
+                            const amlike_matrix_t *residual, const amlike_matrix_t *out, void *stream) {
+  const char *call = "amlike_linear_apply";
+  if (int rc = BindHandle(h)) return rc;
+  if (!h || rows < 0 || activation < AMLIKE_ACT_NONE || activation > AMLIKE_ACT_GELU) {
+    SetError("%s: no handle, %d rows, or unknown activation %d", call, rows, activation);
+    return AMLIKE_EINVAL;
+  }
+  if (int rc = CheckMatrix(call, "x", x, rows, h->k)) return rc;
+  if (int rc = CheckMatrix(call, "out", out, rows, h->n)) return rc;
+  if (residual)
+    if (int rc = CheckMatrix(call, "residual", residual, rows, h->n)) return rc;
+  if (x->type != h->type || (residual && residual->type == AMLIKE_MX8)) {
+    SetError("%s: x has not the layer's type, or the residual is in 8 bits", call);
+    return AMLIKE_EINVAL;
+  }
+  if (rows == 0) return AMLIKE_OK;
+  if (MatricesOverlap(x, rows, h->k, out, rows, h->n) ||
+      (residual && !SameMatrix(residual, out) && MatricesOverlap(residual, rows, h->n, out, rows, h->n))) {
+    SetError("%s: out overlaps an input", call);
+    return AMLIKE_EINVAL;
+  }
+  LinearArgs a = {};
+  a.x = static_cast<const uint8_t *>(x->data);
+  a.x_scales = static_cast<const uint8_t *>(x->scales);
+  a.ldx = x->ld * TypeBytes(x->type);
+  a.ld_xs = x->ld_scales;
+  a.w = h->d_w;
+  a.w_scales = h->d_scales;
+  a.bias = h->d_bias;
+  a.res_type = -1;
+  if (residual) {
+    a.res = residual->data;
+    a.ldr = residual->ld;
+    a.res_type = residual->type;
+  }
+  a.out = out->data;
+  a.out_scales = static_cast<uint8_t *>(out->scales);
+  a.ldo = out->ld;
+  a.ld_os = out->ld_scales;
+  a.out_type = out->type;
+  a.rows = rows;
+  a.k = h->k;
+  a.n = h->n;
+  a.n_pad = h->n_pad;
+  a.k_tiles = h->k_tiles;
+  a.act = activation;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (h->type == AMLIKE_BF16) return LaunchLinear<AMLIKE_BF16>(a, st);
+  if (h->type == AMLIKE_F16) return LaunchLinear<AMLIKE_F16>(a, st);
+  if (out->type == AMLIKE_F32) return LaunchLinear<kMx8Exact>(a, st);
+  return LaunchLinear<AMLIKE_MX8>(a, st);
+}
+
+int amlike_linear_apply(amlike_linear_t *h, const float *x, int32_t ld, int32_t rows, int32_t activation,
+                        const float *residual, int32_t ldr, float *out, int32_t ldo) {
+  if (int rc = BindHandle(h)) return rc;
+  if (!h || !x || !out || rows < 0 || ld < h->k || ldo < h->n || (residual && ldr < h->n)) {
+    SetError("amlike_linear_apply: invalid argument");
+    return AMLIKE_EINVAL;
+  }
+  if (rows == 0) return AMLIKE_OK;
+  std::lock_guard<std::mutex> lock(h->mu);
+  const size_t xrow = (size_t)h->k * sizeof(float), orow = (size_t)h->n * sizeof(float);
+  const int groups = (h->k + 31) / 32;
+  const size_t ldq = ((size_t)h->k + 15) / 16 * 16, values = ldq * TypeBytes(h->type) * rows;
+  int rc = h->ws_x.Reserve(xrow * rows);
+  if (rc == AMLIKE_OK) rc = h->ws_q.Reserve(values + (h->type == AMLIKE_MX8 ? (size_t)groups * rows : 0));
+  if (rc == AMLIKE_OK && residual) rc = h->ws_r.Reserve(orow * rows);
+  if (rc == AMLIKE_OK) rc = h->ws_out.Reserve(orow * rows);
+  if (rc != AMLIKE_OK) return rc;
+  AMLIKE_HIP(hipMemcpy2DAsync(h->ws_x.ptr, xrow, x, (size_t)ld * sizeof(float), xrow, rows, hipMemcpyHostToDevice, h->stream));
+  if (residual)
+    AMLIKE_HIP(hipMemcpy2DAsync(h->ws_r.ptr, orow, residual, (size_t)ldr * sizeof(float), orow, rows, hipMemcpyHostToDevice,
+                                h->stream));
+  const amlike_matrix_t mx = {h->ws_x.ptr, nullptr, h->k, 0, AMLIKE_F32},
+                        mq = {h->ws_q.ptr, h->type == AMLIKE_MX8 ? static_cast<char *>(h->ws_q.ptr) + values : nullptr,
+                              (int64_t)ldq, groups, h->type},
+                        mr = {h->ws_r.ptr, nullptr, h->n, 0, AMLIKE_F32}, mo = {h->ws_out.ptr, nullptr, h->n, 0, AMLIKE_F32};
+  rc = LaunchConvert(mx, rows, h->k, mq, h->stream);
+  if (rc == AMLIKE_OK) rc = amlike_linear_apply_dev(h, &mq, rows, activation, residual ? &mr : nullptr, &mo, h->stream);
+  if (rc != AMLIKE_OK) {
+    (void)hipStreamSynchronize(h->stream);  // the copies above read the caller's arrays
+    return rc;
+  }
+  return CopyMatrixToHost(out, (size_t)ldo, static_cast<const float *>(h->ws_out.ptr), rows, h->n, h->stream);
+}
+
+}  // extern "C"

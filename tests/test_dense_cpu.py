@@ -1,0 +1,91 @@
+"""Refusals of the dense-layer entry points that need no GPU, and the 64-bit references' own checks."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import dense_util as U
+from kaldi_amd import _lib, dense
+
+
+def convert(x, rows, cols, out):
+    return _lib.lib().amlike_convert_dev(x, rows, cols, out, None)
+
+
+def matrix(ptr=4096, type_="bf16", ld=64, scales=0, ld_scales=0):
+    return dense.Matrix(ptr, type_, ld, scales, ld_scales).ref
+
+
+@pytest.mark.parametrize("x,rows,cols,out,text", [
+    (dict(), -1, 64, dict(ptr=1 << 20), "rows"),
+    (dict(), 4, 0, dict(ptr=1 << 20), "columns"),
+    (dict(), 4, (1 << 30) + 1, dict(ptr=1 << 20), "columns"),
+    (dict(ptr=0), 4, 64, dict(ptr=1 << 20), "no data"),
+    (dict(ptr=4097), 4, 64, dict(ptr=1 << 20), "aligned"),
+    (dict(ld=63), 4, 64, dict(ptr=1 << 20), "stride"),
+    (dict(ld=-64), 4, 64, dict(ptr=1 << 20), "stride"),
+    (dict(ld=1 << 60), 4, 64, dict(ptr=1 << 20), "stride"),
+    (dict(), 4, 64, dict(ptr=1 << 20, ld=63), "stride"),
+    (dict(), 4, 64, dict(ptr=1 << 20, type_="mx8"), "scales"),
+    (dict(), 4, 64, dict(ptr=1 << 20, type_="mx8", scales=1 << 21, ld_scales=1), "stride"),
+    (dict(type_="mx8", scales=1 << 21, ld_scales=2), 4, 64, dict(ptr=1 << 20), "8 bits"),
+    (dict(), 4, 64, dict(ptr=4096), "overlap"),
+    (dict(), 4, 64, dict(ptr=4096 + 4 * 64 * 2 - 2), "overlap"),
+    (dict(), 4, 64, dict(ptr=1 << 20, type_="mx8", scales=4100, ld_scales=2), "overlap"),
+])
+def test_convert_refuses(x, rows, cols, out, text):
+    assert convert(matrix(**x), rows, cols, matrix(**out)) == _lib.EINVAL
+    assert text in _lib.lib().amlike_last_error().decode()
+
+
+def test_convert_refuses_unknown_types_and_null():
+    bad = _lib.Matrix(4096, 0, 64, 0, 4)
+    assert convert(ctypes.byref(bad), 4, 64, matrix(ptr=1 << 20)) == _lib.EINVAL
+    bad.type = -1
+    assert convert(matrix(), 4, 64, ctypes.byref(bad)) == _lib.EINVAL
+    assert convert(None, 4, 64, matrix()) == _lib.EINVAL
+    assert convert(matrix(), 4, 64, None) == _lib.EINVAL
+    assert convert(matrix(ptr=0), 0, 64, matrix(ptr=0)) == _lib.OK  # no rows: nothing to look at
+
+
+def test_create_refuses():
+    L, h = _lib.lib(), ctypes.c_void_p()
+    fp = ctypes.POINTER(ctypes.c_float)
+    w = np.ones((4, 8), np.float32)
+    p = w.ctypes.data_as(fp)
+    for args in ((None, 8, None, 8, 4, 1), (p, 7, None, 8, 4, 1), (p, 8, None, 0, 4, 1), (p, 8, None, 8, 0, 1), (p, 8, None, 8, 4, 0),
+                 (p, 8, None, 8, 4, 4), (p, (1 << 20) + 1, None, (1 << 20) + 1, 4, 1), (p, 8, None, 8, (1 << 20) + 1, 1)):
+        assert L.amlike_linear_create(*args, ctypes.byref(h)) == _lib.EINVAL and not h.value
+    assert L.amlike_linear_create(p, 8, None, 8, 4, 1, None) == _lib.EINVAL
+    for dim, eps in ((0, 1e-5), (-1, 1e-5), (32769, 1e-5), (8, 0.0), (8, -1.0), (8, 2.0), (8, math.nan), (8, math.inf), (8, 1e-31)):
+        assert L.amlike_norm_create(None, dim, eps, ctypes.byref(h)) == _lib.EINVAL and not h.value
+    assert L.amlike_norm_create(None, 8, 1e-5, None) == _lib.EINVAL
+    assert L.amlike_norm_destroy(None) == _lib.OK and L.amlike_linear_destroy(None) == _lib.OK
+    assert L.amlike_norm_dim(None) == 0 and L.amlike_linear_output_dim(None) == 0
+    assert L.amlike_norm_device(None) == -1 and L.amlike_linear_device(None) == -1 and L.amlike_linear_type(None) == -1
+
+
+def test_python_mirror_checks_shapes():
+    with pytest.raises(ValueError):
+        dense.Linear(np.ones(3, np.float32))
+    with pytest.raises(ValueError):
+        dense.Linear(np.ones((3, 2), np.float32), np.ones(2, np.float32))
+    with pytest.raises(ValueError):
+        dense.RmsNorm(4, np.ones(3, np.float32))
+    with pytest.raises(KeyError):
+        dense.Matrix(0, "int4", 1)
+
+
+def test_the_reference_of_the_8_bit_form():
+    """Every e4m3 value survives, and a plan of borders gives the scales of the definition."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    codes = codes[(codes & 0x7F) != 0x7F]
+    v = codes.view(torch.float8_e4m3fn).double()
+    x = torch.zeros((len(v), 32), dtype=torch.float64)
+    x[:, 0], x[:, 1] = v, 448.0
+    q, s = U.to_mx8(x)
+    assert torch.equal(U.from_mx8(q, s), x) and (s == 127).all()
+    for top, k in ((448.0, 0), (448.0001, 1), (224.0, -1), (1.75, -8), (1.7501, -7), (2.0 ** 127, 119), (0.0, -127), (2.0 ** -149, -127)):
+        assert int(U.mx8_exponents(torch.full((1, 32), top, dtype=torch.float64))[0, 0]) == k
