@@ -19,6 +19,7 @@
 //   W:      [k-tile][row, physical order, padded to 64][128 bytes], zeros behind both ends
 //   scales: [k-tile][row, the same order][4 bytes], 2^0 behind both ends  (8 bits only)
 #include <algorithm>
+#include <cstdlib>
 #include <mutex>
 #include <new>
 
@@ -240,6 +241,45 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, int64_t m, int n, f
   }
 }
 
+// Sums of sixteen consecutive outputs n .. n + 15 (n a multiple of 16) of row m, biased, become
+// output; lanes l and l ^ 16 hold a group of 32 and both call it.
+__device__ __forceinline__ void finish16(const LinearArgs &a, int64_t m, int n, float v[16]) {
+  const int cols = m < a.rows ? a.n - n : 0;
+  activate<16>(a.act, a.out_type == AMLIKE_F32, v);
+  if (a.res_type >= 0 && cols > 0) {
+    float r[16];
+    load8_any(a.res_type, a.res, m * a.ldr + n, cols, r);
+    load8_any(a.res_type, a.res, m * a.ldr + n + 8, cols - 8, r + 8);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] += r[i];
+  }
+  if (a.out_type == AMLIKE_MX8) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, i < cols ? finite_bits(v[i]) : 0u);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    const int k = mx8_exponent(top);
+    if (cols > 0) {
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = mx8_pack4(v + 4 * i, k);
+      uint8_t *p = static_cast<uint8_t *>(a.out) + m * a.ldo + n;
+      if (cols >= 16) {
+        typedef u32x4 u32x4_byte __attribute__((aligned(1)));
+        *reinterpret_cast<u32x4_byte *>(p) = w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < cols) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+      }
+      if ((n & 31) == 0) a.out_scales[m * a.ld_os + (n >> 5)] = (uint8_t)(k + 127);
+    }
+  } else if (cols > 0) {
+    store8_any(a.out_type, a.out, m * a.ldo + n, cols, v);
+    if (cols > 8) store8_any(a.out_type, a.out, m * a.ldo + n + 8, cols - 8, v + 8);
+  }
+}
+
 // ---- operands ----------------------------------------------------------------------------------------
 
 // Bytes [at, at + 16) of a row of x as columns, those at the row's end `bytes` and beyond as 0.
@@ -334,6 +374,157 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinearArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = s_c[m][c * 8 + j];
     finish8(a, m0 + m, n0 + c * 8, v);
+  }
+}
+
+// ---- the pipelined tile kernel: rows of x that start on 16 bytes ---------------------------------------
+// WN x WM waves, each with 64 outputs x 16 MF rows: 16-byte pieces of the k-tiles go from memory
+// straight into LDS (no registers), those of tile t + 1 while tile t is multiplied.
+
+// Asynchronous copies of 16 (4) bytes per lane: lane l's come from p and go to LDS at `lds` + 16 l
+// (4 l).  Written in assembly so that the compiler, which cannot tell the two halves of the
+// buffer apart, does not make every read of LDS wait for them; they have no result register, and
+// wait_copies ends them.
+__device__ __forceinline__ void copy16_to_lds(const void *p, uint32_t lds) {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ void copy4_to_lds(const void *p, uint32_t lds) {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ void wait_copies() {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#endif
+}
+// Sixteen zero bytes: where pieces behind a row's end come from.
+__device__ u32x4 g_zero_piece;
+
+template <int KIND, int WN, int WM, int MF>
+__global__ __launch_bounds__(64 * WN * WM, 2) void linear_pipe_kernel(LinearArgs a, int m_tiles, int n_tiles) {
+  constexpr int kWaves = WN * WM, BN = 64 * WN, BM = 16 * MF * WM;
+  constexpr bool kMx = IsMx8(KIND);
+  constexpr int kPiecesW = BN * kChunks / (64 * kWaves), kPiecesX = BM * kChunks / (64 * kWaves);  // per wave
+  __shared__ u32x4 s_w[2][BN * kChunks], s_x[2][BM * kChunks];
+  __shared__ uint32_t s_sc[2][kMx ? BN + BM : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
+  const int wn = wave % WN, wm = wave / WN;
+
+  // Blocks go to the 8 dies in turn; each die takes a run of tiles of its own, ordered in bands of
+  // 4 row tiles, so that the 32 tiles a die works on share 4 strips of x and 8 of W in its L2.
+  const int total = m_tiles * n_tiles, die = blockIdx.x & 7, per = total >> 3, more = total & 7;
+  const int lin = die * per + min(die, more) + (blockIdx.x >> 3);
+  const int band = lin / (4 * n_tiles), in = lin - band * 4 * n_tiles, high = min(4, m_tiles - band * 4);
+  const int64_t m0 = (int64_t)(band * 4 + in % high) * BM;
+  const int n0 = in / high * BN;
+  const int bytes = a.k * (kMx ? 1 : 2);
+
+  // This lane's pieces: instruction i of the wave fills 8 rows of the tile, lane l the place l % 8
+  // of row l / 8 (see lds_piece).
+  const uint8_t *pw[kPiecesW], *px[kPiecesX], *psc = nullptr;
+  int cx[kPiecesX];
+#pragma unroll
+  for (int i = 0; i < kPiecesW; ++i) {
+    const int r = (wave * kPiecesW + i) * 8 + (lane >> 3), c = (lane & 7) ^ (r >> 1 & 7);
+    pw[i] = a.w + (int64_t)min(n0 + r, a.n_pad - 1) * kTileBytes + c * 16;
+  }
+#pragma unroll
+  for (int i = 0; i < kPiecesX; ++i) {
+    const int r = (wave * kPiecesX + i) * 8 + (lane >> 3), c = (lane & 7) ^ (r >> 1 & 7);
+    cx[i] = c * 16;
+    px[i] = a.x + min(m0 + r, (int64_t)a.rows - 1) * a.ldx + cx[i];
+  }
+  int64_t step_sc = 0;
+  constexpr int kScWaves = (BN + BM) / 64;  // waves' worth of scale words, W's first
+  constexpr int kScPer = (kScWaves + kWaves - 1) / kWaves;
+  const uint8_t *pscs[kMx ? kScPer : 1];
+  if constexpr (kMx) {
+#pragma unroll
+    for (int i = 0; i < kScPer; ++i) {
+      const int r = (wave + i * kWaves) * 64 + lane;
+      pscs[i] = r < BN ? reinterpret_cast<const uint8_t *>(a.w_scales + min(n0 + r, a.n_pad - 1))
+                       : a.x_scales + min(m0 + r - BN, (int64_t)a.rows - 1) * a.ld_xs;
+    }
+  }
+  const int64_t w_step = (int64_t)a.n_pad * kTileBytes;
+
+  auto fetch = [&](int kt) __attribute__((always_inline)) {
+    const int b = kt & 1;
+    const uint32_t lw = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&s_w[b][wave * kPiecesW * 64];
+    const uint32_t lx = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&s_x[b][wave * kPiecesX * 64];
+#pragma unroll
+    for (int i = 0; i < kPiecesW; ++i) copy16_to_lds(pw[i] + kt * w_step, lw + i * 1024);
+    if ((kt + 1) * kTileBytes <= bytes) {
+#pragma unroll
+      for (int i = 0; i < kPiecesX; ++i) copy16_to_lds(px[i] + kt * kTileBytes, lx + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPiecesX; ++i) {
+        const uint8_t *p = px[i] + kt * kTileBytes;
+        copy16_to_lds(kt * kTileBytes + cx[i] < bytes ? p : reinterpret_cast<const uint8_t *>(&g_zero_piece), lx + i * 1024);
+      }
+    }
+    if constexpr (kMx) {
+#pragma unroll
+      for (int i = 0; i < kScPer; ++i) {
+        const int w = wave + i * kWaves;
+        if (w < kScWaves) {
+          const uint32_t ls = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&s_sc[b][w * 64];
+          copy4_to_lds(pscs[i] + (w < BN / 64 ? (int64_t)kt * a.n_pad * 4 : (int64_t)kt * 4), ls);
+        }
+      }
+    }
+  };
+
+  f32x4v acc[4][MF] = {};
+  fetch(0);
+  for (int kt = 0; kt < a.k_tiles; ++kt) {
+    wait_copies();  // this wave's pieces of tile kt are in LDS, and its reads of tile kt - 1 done
+    __builtin_amdgcn_s_barrier();  // everybody's
+    if (kt + 1 < a.k_tiles) fetch(kt + 1);
+    const int b = kt & 1;
+    const int groups = kMx ? min(4, ((a.k + 31) >> 5) - kt * 4) : 0;
+    auto operand = [&](const u32x4 *tile, const uint32_t *scales, int row) __attribute__((always_inline)) {
+      Operand<KIND> o;
+      uint32_t sc = 0;
+      if constexpr (kMx) {
+        sc = scales[row];
+        if (groups < 4) sc = (sc & ~(~0u << (8 * groups))) | (0x7f7f7f7fu << (8 * groups));  // what lies behind the row's scales
+      }
+      o.set(tile[lds_piece(row, g)], tile[lds_piece(row, g + 4)], sc, g);
+      return o;
+    };
+    Operand<KIND> fw[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) fw[f] = operand(s_w[b], s_sc[b], wn * 64 + f * 16 + r16);
+#pragma unroll
+    for (int e = 0; e < MF; ++e) {
+      const Operand<KIND> fx = operand(s_x[b], s_sc[b] + (kMx ? BN : 0), wm * 16 * MF + e * 16 + r16);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) acc[f][e] = tile_product<KIND>(fw[f], fx, acc[f][e]);
+    }
+  }
+
+  // lane (r16, g): row r16 of fragment e, outputs g * 16 + f * 4 .. + 3 of fragment f: 16 in a row
+  const int n = n0 + wn * 64 + g * 16;
+  float bias[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4v q = n < a.n_pad ? *reinterpret_cast<const f32x4v *>(a.bias + n + 4 * i) : f32x4v{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[4 * i + j] = q[j];
+  }
+#pragma unroll
+  for (int e = 0; e < MF; ++e) {
+    float v[16];
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * f + i] = acc[f][e][i] + bias[4 * f + i];
+    finish16(a, m0 + wm * 16 * MF + e * 16 + r16, n, v);
   }
 }
 
@@ -462,8 +653,33 @@ int ByRows(LinearArgs a, F launch) {
   return AMLIKE_OK;
 }
 
+template <int KIND, int WN, int WM, int MF>
+int LaunchPipe(const LinearArgs &args, hipStream_t st) {
+  return ByRows(args, [&](const LinearArgs &a) -> int {
+    const int m_tiles = (a.rows + 16 * MF * WM - 1) / (16 * MF * WM), n_tiles = (a.n_pad + 64 * WN - 1) / (64 * WN);
+    hipLaunchKernelGGL((linear_pipe_kernel<KIND, WN, WM, MF>), dim3((unsigned)m_tiles * n_tiles), dim3(64 * WN * WM), 0, st, a,
+                       m_tiles, n_tiles);
+    AMLIKE_HIP(hipGetLastError());
+    return AMLIKE_OK;
+  });
+}
+
+// Whether 16-byte pieces of x can be copied as they are: rows start on 16 bytes and end on one (or
+// the last piece would bring what lies behind the row), scales on 4.
+bool Pipeable(const LinearArgs &a, int kind) {
+  const int es = IsMx8(kind) ? 1 : 2;
+  return (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.ldx | (uintptr_t)a.k * es) % 16 == 0 &&
+         (!IsMx8(kind) || (reinterpret_cast<uintptr_t>(a.x_scales) | (uintptr_t)a.ld_xs) % 4 == 0);
+}
+
 template <int TYPE>
 int LaunchLinear(const LinearArgs &args, hipStream_t st) {
+  if (Pipeable(args, TYPE)) {
+    const char *v = getenv("AMLIKE_LIN");
+    const int c = v ? atoi(v) : args.rows >= 2048 ? 1 : 2;
+    if (c == 1) return LaunchPipe<TYPE, 4, 2, 8>(args, st);
+    if (c == 2) return LaunchPipe<TYPE, 2, 2, 4>(args, st);
+  }
   return ByRows(args, [&](const LinearArgs &a) -> int {
     const int64_t tiles = ((int64_t)a.rows + 63) / 64 * (a.n_pad / 64);
     hipLaunchKernelGGL(linear_tile_kernel<TYPE>, dim3((unsigned)tiles), dim3(256), 0, st, a);
