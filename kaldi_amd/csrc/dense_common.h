@@ -39,6 +39,7 @@ typedef u32x2 u32x2_any __attribute__((aligned(1)));
 
 // (By value: __builtin_bit_cast of a vector's element reads element 0 whichever is named.)
 __device__ __forceinline__ float as_float(uint32_t w) { return __builtin_bit_cast(float, w); }
+__device__ __forceinline__ uint32_t as_bits(float v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ f16x2v as_f16x2(uint32_t w) { return __builtin_bit_cast(f16x2v, w); }
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }

@@ -7,19 +7,17 @@
 // fragment holds row l % 16 and, of its k-tile, the 32 bytes l / 16 -- the 16-bit ones as two
 // instructions of 16 bytes each (which columns meet in one instruction does not matter as long as
 // both operands agree), the 8-bit one as a single instruction whose scale is that lane's byte.
-// W is the instructions' first operand and x the second, so that a lane's results are 4
-// consecutive outputs of one row of x per fragment; rows of W are stored in an order (PhysicalRow)
-// that makes them 16 consecutive outputs over four fragments.
+// W is the instructions' first operand and x the second, so that a lane's results are 4 outputs of
+// one row of x per fragment.
 // The 8-bit instruction aligns the products of a few neighbouring columns to the largest of them
 // and drops what lies more than 13 binary places below it (measured: 2^16 + 2^2 is 2^16, 2^16 + 2^3
 // is whole), which leaves a relative error of about 1.5e-5 in a sum of normal values whatever its
 // length: far below the rounding of a 16-bit (2^-9, 2^-12 on average) or 8-bit output, too much for
 // an fp32 one.  For an fp32 output the 8-bit operands are therefore widened to bf16, which holds
 // value times scale exactly, and multiplied there (kMx8Exact), at half the matrix rate.
-//   W:      [k-tile][row, physical order, padded to 64][128 bytes], zeros behind both ends
-//   scales: [k-tile][row, the same order][4 bytes], 2^0 behind both ends  (8 bits only)
+//   W:      [k-tile][row, padded to 64][128 bytes], zeros behind both ends
+//   scales: [k-tile][row, padded to 64][4 bytes], 2^0 behind both ends  (8 bits only)
 #include <algorithm>
-#include <cstdlib>
 #include <mutex>
 #include <new>
 
@@ -30,10 +28,6 @@ namespace amlike {
 constexpr int kTileBytes = 128;  // of a row in a k-tile
 constexpr int kChunks = 8;       // 16-byte pieces of it
 constexpr int kLinearMaxDim = 1 << 20;   // either dimension of a layer
-
-// Within 64 outputs: where output n = g * 16 + f * 4 + i is stored: row f * 16 + g * 4 + i, row
-// g * 4 + i of fragment f.  The map is its own inverse.
-__host__ __device__ constexpr int PhysicalRow(int n) { return (n & ~63) | (n & 3) | (n >> 2 & 12) | (n << 2 & 48); }
 
 struct LinearArgs {
   const uint8_t *x, *x_scales;  // [rows][k], row strides in bytes
@@ -171,34 +165,31 @@ __device__ __forceinline__ float fast_tanh(float x) {
 
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-x)); }
 
-template <int N>
-__device__ __forceinline__ void activate(int act, bool exact, float *v) {
-  if (act == AMLIKE_ACT_NONE) return;
-  if (act == AMLIKE_ACT_RELU) {  // (a comparison: NaN stays)
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
-  } else if (act == AMLIKE_ACT_SIGMOID) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = sigmoid(v[i]);
-  } else if (act == AMLIKE_ACT_TANH) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = fast_tanh(v[i]);
-  } else if (act == AMLIKE_ACT_SILU) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] *= sigmoid(v[i]);
-  } else if (exact) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float q = normal_tail<true>(__builtin_fabsf(v[i]));
-      v[i] *= v[i] > 0.0f ? 1.0f - q : q;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float q = normal_tail<false>(__builtin_fabsf(v[i]));
-      v[i] *= v[i] > 0.0f ? 1.0f - q : q;
-    }
+// One value; EXACT: for an fp32 output.  (relu is a comparison: NaN stays.)
+template <int ACT, bool EXACT>
+__device__ __forceinline__ float activated(float x) {
+  if constexpr (ACT == AMLIKE_ACT_RELU) return x < 0.0f ? 0.0f : x;
+  if constexpr (ACT == AMLIKE_ACT_SIGMOID) return sigmoid(x);
+  if constexpr (ACT == AMLIKE_ACT_TANH) return fast_tanh(x);
+  if constexpr (ACT == AMLIKE_ACT_SILU) return x * sigmoid(x);
+  if constexpr (ACT == AMLIKE_ACT_GELU) {
+    const float q = normal_tail<EXACT>(__builtin_fabsf(x));
+    return x * (x > 0.0f ? 1.0f - q : q);
   }
+  return x;
+}
+// F(integral_constant-like tag) for the activation that the arguments name.
+template <int ACT>
+struct ActTag {
+  static constexpr int value = ACT;
+};
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+  if (act == AMLIKE_ACT_RELU) f(ActTag<AMLIKE_ACT_RELU>());
+  else if (act == AMLIKE_ACT_SIGMOID) f(ActTag<AMLIKE_ACT_SIGMOID>());
+  else if (act == AMLIKE_ACT_TANH) f(ActTag<AMLIKE_ACT_TANH>());
+  else if (act == AMLIKE_ACT_SILU) f(ActTag<AMLIKE_ACT_SILU>());
+  else if (act == AMLIKE_ACT_GELU) f(ActTag<AMLIKE_ACT_GELU>());
 }
 
 __device__ __forceinline__ uint32_t quad_max_bits(uint32_t u) {
@@ -218,7 +209,11 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, int64_t m, int n, f
       v[i] += b0[i];
       v[4 + i] += b1[i];
     }
-    activate<8>(a.act, a.out_type == AMLIKE_F32, v);
+    with_activation(a.act, [&](auto tag) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = a.out_type == AMLIKE_F32 ? activated<decltype(tag)::value, true>(v[i]) : activated<decltype(tag)::value, false>(v[i]);
+    });
     if (a.res_type >= 0) {
       float r[8];
       load8_any(a.res_type, a.res, m * a.ldr + n, cols, r);
@@ -241,30 +236,89 @@ __device__ __forceinline__ void finish8(const LinearArgs &a, int64_t m, int n, f
   }
 }
 
-// Sums of sixteen consecutive outputs n .. n + 15 (n a multiple of 16) of row m, biased, become
-// output; lanes l and l ^ 16 hold a group of 32 and both call it.
-__device__ __forceinline__ void finish16(const LinearArgs &a, int64_t m, int n, float v[16]) {
-  const int cols = m < a.rows ? a.n - n : 0;
-  activate<16>(a.act, a.out_type == AMLIKE_F32, v);
-  if (a.res_type >= 0 && cols > 0) {
+// A wave's 64 outputs over its four fragments of W, so dealt that a lane (r16, g) stores 16 bytes at
+// a time and four lanes store 64 in a row: CH consecutive outputs per lane, 4 in fp32, 8 in 16 bits,
+// 16 in 8.  Value 4 f + i of the lane (register i of fragment f) is element i of chunk ...
+template <int CH>
+__device__ __forceinline__ int chunk_output(int j, int g) { return j * (4 * CH) + g * CH; }  // of chunk j = value / CH
+// ... so row rho of fragment f of W is output
+__device__ __forceinline__ int fragment_output(int ch, int f, int rho) {
+  const int per = ch >> 2;  // fragments per chunk
+  return (f / per) * (4 * ch) + (rho >> 2) * ch + (f % per) * 4 + (rho & 3);
+}
+
+// The biases of a lane's 16 outputs.
+template <int CH>
+__device__ __forceinline__ void load_bias(const LinearArgs &a, int n, int g, f32x4v bias[4]) {
+#pragma unroll
+  for (int f = 0; f < 4; ++f) {
+    const int at = n + chunk_output<CH>(4 * f / CH, g) + 4 * f % CH;
+    bias[f] = *reinterpret_cast<const f32x4v *>(a.bias + min(at, a.n_pad - 4));  // (behind the end: of no output)
+  }
+}
+
+// CH consecutive elements of a row as CH floats, all there.
+template <int CH, int TYPE>
+__device__ __forceinline__ void load_chunk_of(const void *data, int64_t at, float *v) {
+  if constexpr (CH == 4 && TYPE == AMLIKE_F32) {
+    const u32x4 q = *reinterpret_cast<const u32x4_f *>(static_cast<const float *>(data) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = as_float(q[i]);
+  } else if constexpr (CH == 4) {
+    typedef u32x2 u32x2_half __attribute__((aligned(2)));
+    const u32x2 q = *reinterpret_cast<const u32x2_half *>(static_cast<const uint16_t *>(data) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = q[i >> 1];
+      v[i] = TYPE == AMLIKE_BF16 ? (i & 1 ? bf16_hi(w) : bf16_lo(w)) : (float)as_f16x2(w)[i & 1];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CH; i += 8) load8<TYPE>(data, at + i, 8, v + i);
+  }
+}
+
+// The 16 activated sums of a lane for a row become output; n is the wave's first output.  INNER: all
+// 64 exist; otherwise the elements go one by one.
+template <int CH, bool INNER>
+__device__ __forceinline__ void finish_row(const LinearArgs &a, int64_t row, int n, int g, float v[16]) {
+  const bool live = row < a.rows;
+  if (a.res_type >= 0 && live) {
     float r[16];
-    load8_any(a.res_type, a.res, m * a.ldr + n, cols, r);
-    load8_any(a.res_type, a.res, m * a.ldr + n + 8, cols - 8, r + 8);
+    if constexpr (INNER) {
+      auto load = [&](auto tag) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 16 / CH; ++j)
+          load_chunk_of<CH, decltype(tag)::value>(a.res, row * a.ldr + n + chunk_output<CH>(j, g), r + j * CH);
+      };
+      if (a.res_type == AMLIKE_F32) load(ActTag<AMLIKE_F32>());
+      else if (a.res_type == AMLIKE_BF16) load(ActTag<AMLIKE_BF16>());
+      else load(ActTag<AMLIKE_F16>());
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = n + chunk_output<CH>(i / CH, g) + i % CH;
+        float one[8] = {0};
+        if (at < a.n) load8_any(a.res_type, a.res, row * a.ldr + at, 1, one);
+        r[i] = one[0];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] += r[i];
   }
-  if (a.out_type == AMLIKE_MX8) {
+  if constexpr (CH == 16) {
+    const int at = n + chunk_output<16>(0, g), cols = INNER ? 16 : a.n - at;
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = max(top, i < cols ? finite_bits(v[i]) : 0u);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));  // lanes l and l ^ 16 hold a group of 32
     const int k = mx8_exponent(top);
-    if (cols > 0) {
+    if (live && cols > 0) {
       u32x4 w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = mx8_pack4(v + 4 * i, k);
-      uint8_t *p = static_cast<uint8_t *>(a.out) + m * a.ldo + n;
-      if (cols >= 16) {
+      uint8_t *p = static_cast<uint8_t *>(a.out) + row * a.ldo + at;
+      if (INNER || cols >= 16) {
         typedef u32x4 u32x4_byte __attribute__((aligned(1)));
         *reinterpret_cast<u32x4_byte *>(p) = w;
       } else {
@@ -272,11 +326,61 @@ __device__ __forceinline__ void finish16(const LinearArgs &a, int64_t m, int n, 
         for (int i = 0; i < 16; ++i)
           if (i < cols) p[i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
       }
-      if ((n & 31) == 0) a.out_scales[m * a.ld_os + (n >> 5)] = (uint8_t)(k + 127);
+      if ((g & 1) == 0) a.out_scales[row * a.ld_os + (at >> 5)] = (uint8_t)(k + 127);
     }
-  } else if (cols > 0) {
-    store8_any(a.out_type, a.out, m * a.ldo + n, cols, v);
-    if (cols > 8) store8_any(a.out_type, a.out, m * a.ldo + n + 8, cols - 8, v + 8);
+  } else if (live) {
+    if constexpr (INNER) {
+#pragma unroll
+      for (int j = 0; j < 16 / CH; ++j) {
+        const int64_t to = row * a.ldo + n + chunk_output<CH>(j, g);
+        const float *q = v + j * CH;
+        if constexpr (CH == 4)
+          *reinterpret_cast<u32x4_f *>(static_cast<float *>(a.out) + to) = u32x4{as_bits(q[0]), as_bits(q[1]), as_bits(q[2]), as_bits(q[3])};
+        else if (a.out_type == AMLIKE_BF16) store8<AMLIKE_BF16>(a.out, to, 8, q);
+        else store8<AMLIKE_F16>(a.out, to, 8, q);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int at = n + chunk_output<CH>(i / CH, g) + i % CH;
+        float one[8] = {v[i]};
+        if (at < a.n) store8_any(a.out_type, a.out, row * a.ldo + at, 1, one);
+      }
+    }
+  }
+}
+
+// All of a wave's rows: fragments E, E + 1 .. of x, from row m of the output on.  (A recursion, not
+// a loop: the registers have to be named, and the compiler gives up unrolling a body of this size.)
+template <bool F32_ONLY, int MF, int E = 0>
+__device__ __forceinline__ void finish_wave(const LinearArgs &a, int64_t m, int n, int r16, int g, const f32x4v acc[4][MF]) {
+  if constexpr (E < MF) {
+    const bool inner = n + 64 <= a.n;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = acc[i >> 2][E][i & 3];
+    with_activation(a.act, [&](auto tag) __attribute__((always_inline)) {
+      constexpr int kAct = decltype(tag)::value;
+      if (kAct == AMLIKE_ACT_GELU && a.out_type != AMLIKE_F32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = activated<kAct, false>(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = activated<kAct, true>(v[i]);
+      }
+    });
+    const int64_t row = m + E * 16 + r16;
+    if (F32_ONLY || a.out_type == AMLIKE_F32) {
+      if (inner) finish_row<4, true>(a, row, n, g, v);
+      else finish_row<4, false>(a, row, n, g, v);
+    } else if (a.out_type == AMLIKE_MX8) {
+      if (inner) finish_row<16, true>(a, row, n, g, v);
+      else finish_row<16, false>(a, row, n, g, v);
+    } else {
+      if (inner) finish_row<8, true>(a, row, n, g, v);
+      else finish_row<8, false>(a, row, n, g, v);
+    }
+    finish_wave<F32_ONLY, MF, E + 1>(a, m, n, r16, g, acc);
   }
 }
 
@@ -304,8 +408,13 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t *row, int kt, int 
 }
 
 // Where 16-byte piece c of row r of a tile lies in LDS: pieces of neighbouring rows are turned
-// against each other, so that 16 lanes reading the same piece of 16 rows meet all banks.
-__device__ __forceinline__ int lds_piece(int r, int c) { return r * kChunks + (c ^ (r >> 1 & 7)); }
+// against each other, so that 16 lanes reading the same piece of 16 rows meet all banks.  For W the
+// 16 rows may be neighbours or dealt as fragment_output has it: bits 0-3, 0 1 3 4 or 0 1 4 5 of r
+// vary, and in each case bits 1-3 of the turn take all values.
+__device__ __forceinline__ int turn_x(int r) { return r >> 1 & 7; }
+__device__ __forceinline__ int turn_w(int r) { return (r >> 1 & 7) ^ (r >> 3 & 6); }
+__device__ __forceinline__ int lds_piece(int r, int c) { return r * kChunks + (c ^ turn_x(r)); }
+__device__ __forceinline__ int lds_piece_w(int r, int c) { return r * kChunks + (c ^ turn_w(r)); }
 
 // ---- the plain tile kernel: any size, alignment and type ----------------------------------------------
 // 64 x 64 outputs per block of four waves (32 x 32 each); k-tiles go through registers into LDS.
@@ -360,12 +469,12 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinearArgs a) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) acc[f][e] = tile_product<TYPE>(fw[f], fx[e], acc[f][e]);
   }
-  // lane (r16, g): row r16 of fragment e of x; of fragment wn / 16 + f of W outputs g * 16 + that * 4 ..
+  // lane (r16, g): row r16 of fragment e of x, outputs g * 4 .. + 3 of fragment f of W
 #pragma unroll
   for (int f = 0; f < 2; ++f)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<f32x4v *>(&s_c[wm + e * 16 + r16][g * 16 + (wn / 16 + f) * 4]) = acc[f][e];
+      *reinterpret_cast<f32x4v *>(&s_c[wm + e * 16 + r16][wn + f * 16 + g * 4]) = acc[f][e];
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -381,24 +490,38 @@ __global__ __launch_bounds__(256) void linear_tile_kernel(LinearArgs a) {
 // WN x WM waves, each with 64 outputs x 16 MF rows: 16-byte pieces of the k-tiles go from memory
 // straight into LDS (no registers), those of tile t + 1 while tile t is multiplied.
 
-// Asynchronous copies of 16 (4) bytes per lane: lane l's come from p and go to LDS at `lds` + 16 l
-// (4 l).  Written in assembly so that the compiler, which cannot tell the two halves of the
+// Asynchronous copies of 16 (4) bytes per lane: lane l's come from base + offset and go to LDS at
+// `lds` + 16 l (4 l).  Written in assembly so that the compiler, which cannot tell the two halves of the
 // buffer apart, does not make every read of LDS wait for them; they have no result register, and
 // wait_copies ends them.
-__device__ __forceinline__ void copy16_to_lds(const void *p, uint32_t lds) {
+__device__ __forceinline__ void copy16_to_lds(const uint8_t *base, uint32_t offset, uint32_t lds) {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+#endif
+}
+__device__ __forceinline__ void copy16_to_lds(const uint8_t *p, uint32_t lds) {  // any address per lane
 #if __HIP_DEVICE_COMPILE__
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 #endif
 }
-__device__ __forceinline__ void copy4_to_lds(const void *p, uint32_t lds) {
+__device__ __forceinline__ void copy4_to_lds(const uint8_t *base, uint32_t offset, uint32_t lds) {
 #if __HIP_DEVICE_COMPILE__
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 #endif
 }
 __device__ __forceinline__ void wait_copies() {
 #if __HIP_DEVICE_COMPILE__
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 #endif
+}
+__device__ __forceinline__ void wait_lds() {
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#endif
+}
+template <typename T>
+__device__ __forceinline__ uint32_t lds_address(T *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)p;
 }
 // Sixteen zero bytes: where pieces behind a row's end come from.
 __device__ u32x4 g_zero_piece;
@@ -413,118 +536,161 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void linear_pipe_kernel(LinearArgs
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, g = lane >> 4;
   const int wn = wave % WN, wm = wave / WN;
 
-  // Blocks go to the 8 dies in turn; each die takes a run of tiles of its own, ordered in bands of
-  // 4 row tiles, so that the 32 tiles a die works on share 4 strips of x and 8 of W in its L2.
+  // Blocks go to the 8 dies in turn; each die takes a run of tiles of its own, which its blocks go
+  // through side by side, ordered in bands of 4 row tiles: the 32 tiles that a die works on share
+  // 4 strips of x and 8 of W in its L2.
   const int total = m_tiles * n_tiles, die = blockIdx.x & 7, per = total >> 3, more = total & 7;
-  const int lin = die * per + min(die, more) + (blockIdx.x >> 3);
-  const int band = lin / (4 * n_tiles), in = lin - band * 4 * n_tiles, high = min(4, m_tiles - band * 4);
-  const int64_t m0 = (int64_t)(band * 4 + in % high) * BM;
-  const int n0 = in / high * BN;
+  const int end = die * per + min(die, more) + per + (die < more ? 1 : 0), stride = gridDim.x >> 3;
+  int lin = die * per + min(die, more) + (blockIdx.x >> 3);
+  if (lin >= end) return;
   const int bytes = a.k * (kMx ? 1 : 2);
-
-  // This lane's pieces: instruction i of the wave fills 8 rows of the tile, lane l the place l % 8
-  // of row l / 8 (see lds_piece).
-  const uint8_t *pw[kPiecesW], *px[kPiecesX], *psc = nullptr;
-  int cx[kPiecesX];
-#pragma unroll
-  for (int i = 0; i < kPiecesW; ++i) {
-    const int r = (wave * kPiecesW + i) * 8 + (lane >> 3), c = (lane & 7) ^ (r >> 1 & 7);
-    pw[i] = a.w + (int64_t)min(n0 + r, a.n_pad - 1) * kTileBytes + c * 16;
-  }
-#pragma unroll
-  for (int i = 0; i < kPiecesX; ++i) {
-    const int r = (wave * kPiecesX + i) * 8 + (lane >> 3), c = (lane & 7) ^ (r >> 1 & 7);
-    cx[i] = c * 16;
-    px[i] = a.x + min(m0 + r, (int64_t)a.rows - 1) * a.ldx + cx[i];
-  }
-  int64_t step_sc = 0;
-  constexpr int kScWaves = (BN + BM) / 64;  // waves' worth of scale words, W's first
-  constexpr int kScPer = (kScWaves + kWaves - 1) / kWaves;
-  const uint8_t *pscs[kMx ? kScPer : 1];
-  if constexpr (kMx) {
-#pragma unroll
-    for (int i = 0; i < kScPer; ++i) {
-      const int r = (wave + i * kWaves) * 64 + lane;
-      pscs[i] = r < BN ? reinterpret_cast<const uint8_t *>(a.w_scales + min(n0 + r, a.n_pad - 1))
-                       : a.x_scales + min(m0 + r - BN, (int64_t)a.rows - 1) * a.ld_xs;
-    }
-  }
   const int64_t w_step = (int64_t)a.n_pad * kTileBytes;
 
-  auto fetch = [&](int kt) __attribute__((always_inline)) {
-    const int b = kt & 1;
-    const uint32_t lw = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&s_w[b][wave * kPiecesW * 64];
-    const uint32_t lx = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&s_x[b][wave * kPiecesX * 64];
+  // This lane's pieces of a tile: instruction i of the wave fills 8 rows of it, lane l the place l % 8
+  // of row l / 8 (see turn_x, turn_w).  Bases are the wave's, in scalar registers.  A wave's rows of W
+  // all lie before or all behind the padded end (they are then read from the wave's first tile's, of
+  // no output); rows of x behind the last are read as the last.
+  constexpr int kRowsW = kPiecesW * 8, kRowsX = kPiecesX * 8;
+  constexpr int kScWaves = (BN + BM) / 64;  // waves' worth of scale words, W's first
+  constexpr int kScPer = (kScWaves + kWaves - 1) / kWaves;
+  static_assert(64 % kRowsW == 0, "a wave's rows of W lie in one 64");
+  int64_t m0;
+  int n0;
+  const uint8_t *bw, *bx, *bsc[kMx ? kScPer : 1];
+  uint32_t ow[kPiecesW], ox[kPiecesX], osc[kMx ? kScPer : 1];
 #pragma unroll
-    for (int i = 0; i < kPiecesW; ++i) copy16_to_lds(pw[i] + kt * w_step, lw + i * 1024);
-    if ((kt + 1) * kTileBytes <= bytes) {
+  for (int i = 0; i < kPiecesW; ++i) {
+    const int r = i * 8 + (lane >> 3);
+    ow[i] = r * kTileBytes + ((lane & 7) ^ turn_w(wave * kRowsW + r)) * 16;
+  }
+  auto place = [&]() __attribute__((always_inline)) {
+    const int band = lin / (4 * n_tiles), in = lin - band * 4 * n_tiles, high = min(4, m_tiles - band * 4);
+    m0 = (int64_t)(band * 4 + in % high) * BM;
+    n0 = in / high * BN;
+    const int wrow = n0 + wave * kRowsW;
+    bw = a.w + (int64_t)(wrow < a.n_pad ? wrow : 0) * kTileBytes;
+    bx = a.x + m0 * a.ldx;
+    const int last = (int)min((int64_t)BM, a.rows - m0) - 1;
 #pragma unroll
-      for (int i = 0; i < kPiecesX; ++i) copy16_to_lds(px[i] + kt * kTileBytes, lx + i * 1024);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPiecesX; ++i) {
-        const uint8_t *p = px[i] + kt * kTileBytes;
-        copy16_to_lds(kt * kTileBytes + cx[i] < bytes ? p : reinterpret_cast<const uint8_t *>(&g_zero_piece), lx + i * 1024);
-      }
+    for (int i = 0; i < kPiecesX; ++i) {
+      const int r = wave * kRowsX + i * 8 + (lane >> 3);
+      ox[i] = (uint32_t)min(r, last) * (uint32_t)a.ldx + ((lane & 7) ^ turn_x(r)) * 16;
     }
     if constexpr (kMx) {
 #pragma unroll
       for (int i = 0; i < kScPer; ++i) {
-        const int w = wave + i * kWaves;
-        if (w < kScWaves) {
-          const uint32_t ls = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)&s_sc[b][w * 64];
-          copy4_to_lds(pscs[i] + (w < BN / 64 ? (int64_t)kt * a.n_pad * 4 : (int64_t)kt * 4), ls);
+        const int r = (wave + i * kWaves) * 64;  // the wave's first
+        if (r < BN) {
+          bsc[i] = reinterpret_cast<const uint8_t *>(a.w_scales + (n0 + r < a.n_pad ? n0 + r : 0));
+          osc[i] = lane * 4;
+        } else {
+          bsc[i] = a.x_scales + m0 * a.ld_xs;
+          osc[i] = (uint32_t)min(r - BN + lane, last) * (uint32_t)a.ld_xs;
         }
       }
     }
   };
 
-  f32x4v acc[4][MF] = {};
-  fetch(0);
-  for (int kt = 0; kt < a.k_tiles; ++kt) {
-    wait_copies();  // this wave's pieces of tile kt are in LDS, and its reads of tile kt - 1 done
-    __builtin_amdgcn_s_barrier();  // everybody's
-    if (kt + 1 < a.k_tiles) fetch(kt + 1);
+  auto fetch = [&](int kt) __attribute__((always_inline)) {
     const int b = kt & 1;
-    const int groups = kMx ? min(4, ((a.k + 31) >> 5) - kt * 4) : 0;
-    auto operand = [&](const u32x4 *tile, const uint32_t *scales, int row) __attribute__((always_inline)) {
-      Operand<KIND> o;
-      uint32_t sc = 0;
-      if constexpr (kMx) {
-        sc = scales[row];
-        if (groups < 4) sc = (sc & ~(~0u << (8 * groups))) | (0x7f7f7f7fu << (8 * groups));  // what lies behind the row's scales
+    const uint32_t lw = lds_address(&s_w[b][wave * kPiecesW * 64]), lx = lds_address(&s_x[b][wave * kPiecesX * 64]);
+    const uint8_t *w = bw + kt * w_step, *x = bx + kt * kTileBytes;
+#pragma unroll
+    for (int i = 0; i < kPiecesW; ++i) copy16_to_lds(w, ow[i], lw + i * 1024);
+    if ((kt + 1) * kTileBytes <= bytes) {
+#pragma unroll
+      for (int i = 0; i < kPiecesX; ++i) copy16_to_lds(x, ox[i], lx + i * 1024);
+    } else {  // the last k-tile, short: zeros behind the rows' end
+#pragma unroll
+      for (int i = 0; i < kPiecesX; ++i) {
+        const int r = wave * kRowsX + i * 8 + (lane >> 3), at = kt * kTileBytes + ((lane & 7) ^ turn_x(r)) * 16;
+        copy16_to_lds(at < bytes ? x + ox[i] : reinterpret_cast<const uint8_t *>(&g_zero_piece), lx + i * 1024);
       }
-      o.set(tile[lds_piece(row, g)], tile[lds_piece(row, g + 4)], sc, g);
-      return o;
-    };
-    Operand<KIND> fw[4];
-#pragma unroll
-    for (int f = 0; f < 4; ++f) fw[f] = operand(s_w[b], s_sc[b], wn * 64 + f * 16 + r16);
-#pragma unroll
-    for (int e = 0; e < MF; ++e) {
-      const Operand<KIND> fx = operand(s_x[b], s_sc[b] + (kMx ? BN : 0), wm * 16 * MF + e * 16 + r16);
-#pragma unroll
-      for (int f = 0; f < 4; ++f) acc[f][e] = tile_product<KIND>(fw[f], fx, acc[f][e]);
     }
-  }
+    if constexpr (kMx) {
+#pragma unroll
+      for (int i = 0; i < kScPer; ++i) {
+        const int q = wave + i * kWaves;
+        if (q < kScWaves) copy4_to_lds(bsc[i] + (int64_t)kt * (q < BN / 64 ? a.n_pad * 4 : 4), osc[i], lds_address(&s_sc[b][q * 64]));
+      }
+    }
+  };
 
-  // lane (r16, g): row r16 of fragment e, outputs g * 16 + f * 4 .. + 3 of fragment f: 16 in a row
-  const int n = n0 + wn * 64 + g * 16;
-  float bias[16];
+  const int ch = KIND == kMx8Exact || a.out_type == AMLIKE_F32 ? 4 : a.out_type == AMLIKE_MX8 ? 16 : 8;
+  int row_w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f32x4v q = n < a.n_pad ? *reinterpret_cast<const f32x4v *>(a.bias + n + 4 * i) : f32x4v{0, 0, 0, 0};
+  for (int f = 0; f < 4; ++f) row_w[f] = wn * 64 + fragment_output(ch, f, r16);
+
+  // A tile's first two k-tiles and its biases, on their way while the tile before is stored.  The
+  // memory unit answers in order: when the biases are there, so are the k-tiles.
+  f32x4v bias[4];
+  auto start = [&]() __attribute__((always_inline)) {
+    place();
+    fetch(0);
+    if (a.k_tiles > 1) fetch(1);
+    const int n = n0 + wn * 64;
+    if (ch == 4) load_bias<4>(a, n, g, bias);
+    else if (ch == 16) load_bias<16>(a, n, g, bias);
+    else load_bias<8>(a, n, g, bias);
+  };
+
+  start();
+  for (;;) {
+    f32x4v acc[4][MF];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bias[4 * i + j] = q[j];
-  }
+    for (int f = 0; f < 4; ++f) {
+#if __HIP_DEVICE_COMPILE__
+      asm volatile("" : "+v"(bias[f])::"memory");  // the biases are there
+#endif
 #pragma unroll
-  for (int e = 0; e < MF; ++e) {
-    float v[16];
+      for (int e = 0; e < MF; ++e) acc[f][e] = bias[f];
+    }
+    int kt = 0;
+#if __HIP_DEVICE_COMPILE__
+    asm volatile("" : "+s"(kt));  // (one copy of the loop's body: the first k-tiles are not to be peeled off)
+#endif
+#pragma clang loop unroll(disable)
+    for (; kt < a.k_tiles; ++kt) {
+      if (kt < 2) wait_lds();
+      else wait_copies();            // this wave's pieces of tile kt are in LDS, and its reads of tile kt - 1 done
+      __builtin_amdgcn_s_barrier();  // everybody's
+      if (kt >= 1 && kt + 1 < a.k_tiles) fetch(kt + 1);
+      const int b = kt & 1;
+      const int groups = kMx ? min(4, ((a.k + 31) >> 5) - kt * 4) : 0;
+      auto operand = [&](const u32x4 *tile, const uint32_t *scales, int row, int turn) __attribute__((always_inline)) {
+        Operand<KIND> o;
+        uint32_t sc = 0;
+        if constexpr (kMx) {
+          sc = scales[row];
+          if (groups < 4) sc = (sc & ~(~0u << (8 * groups))) | (0x7f7f7f7fu << (8 * groups));  // what lies behind the row's scales
+        }
+        o.set(tile[row * kChunks + (g ^ turn)], tile[row * kChunks + (g ^ 4 ^ turn)], sc, g);
+        return o;
+      };
+      Operand<KIND> fw[4];
 #pragma unroll
-    for (int f = 0; f < 4; ++f)
+      for (int f = 0; f < 4; ++f) fw[f] = operand(s_w[b], s_sc[b], row_w[f], turn_w(row_w[f]));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * f + i] = acc[f][e][i] + bias[4 * f + i];
-    finish16(a, m0 + wm * 16 * MF + e * 16 + r16, n, v);
+      for (int e = 0; e < MF; ++e) {
+        const Operand<KIND> fx = operand(s_x[b], s_sc[b] + (kMx ? BN : 0), wm * 16 * MF + e * 16 + r16, turn_x(r16));
+#pragma unroll
+        for (int f = 0; f < 4; ++f) acc[f][e] = tile_product<KIND>(fw[f], fx, acc[f][e]);
+      }
+    }
+    const int64_t m = m0 + wm * 16 * MF;
+    const int n = n0 + wn * 64;
+    lin += stride;
+    if (lin < end) {
+      wait_lds();
+      __builtin_amdgcn_s_barrier();  // both halves of the buffer are free
+      start();
+    }
+    int er = r16, eg = g;
+#if __HIP_DEVICE_COMPILE__
+    asm volatile("" : "+v"(er), "+v"(eg));  // (or the compiler keeps every address of the epilogue through the k-tiles)
+#endif
+    finish_wave<KIND == kMx8Exact, MF>(a, m, n, er, eg, acc);
+    if (lin >= end) break;
   }
 }
 
@@ -537,7 +703,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint8_t *__restr
   for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < pieces; p += (int64_t)gridDim.x * 256) {
     const int c = (int)(p & 7);
     const int64_t tr = p >> 3;
-    const int kt = (int)(tr / n_pad), row = PhysicalRow((int)(tr - (int64_t)kt * n_pad));
+    const int kt = (int)(tr / n_pad), row = (int)(tr - (int64_t)kt * n_pad);
     const int es = type == AMLIKE_MX8 ? 1 : 2;
     u32x4 q = {0, 0, 0, 0};
     if (row < n) q = load_chunk(src + (int64_t)row * k * es, kt * kTileBytes + c * 16, k * es);
@@ -560,7 +726,7 @@ __global__ __launch_bounds__(256) void linear_pack_scales_kernel(const uint8_t *
                                                                  int64_t words, uint32_t *__restrict__ dst) {
   const int groups = (k + 31) >> 5;
   for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < words; p += (int64_t)gridDim.x * 256) {
-    const int kt = (int)(p / n_pad), row = PhysicalRow((int)(p - (int64_t)kt * n_pad));
+    const int kt = (int)(p / n_pad), row = (int)(p - (int64_t)kt * n_pad);
     dst[p] = row < n ? load_scales(src + (int64_t)row * groups, kt, groups) : 0x7f7f7f7fu;
   }
 }
@@ -657,32 +823,43 @@ template <int KIND, int WN, int WM, int MF>
 int LaunchPipe(const LinearArgs &args, hipStream_t st) {
   return ByRows(args, [&](const LinearArgs &a) -> int {
     const int m_tiles = (a.rows + 16 * MF * WM - 1) / (16 * MF * WM), n_tiles = (a.n_pad + 64 * WN - 1) / (64 * WN);
-    hipLaunchKernelGGL((linear_pipe_kernel<KIND, WN, WM, MF>), dim3((unsigned)m_tiles * n_tiles), dim3(64 * WN * WM), 0, st, a,
-                       m_tiles, n_tiles);
+    // as many blocks as the device holds at once (8 waves a block: one per compute unit), in eights
+    const int held = std::max(8, NumComputeUnits() * 8 / (WN * WM) & ~7);
+    hipLaunchKernelGGL((linear_pipe_kernel<KIND, WN, WM, MF>), dim3((unsigned)std::min((m_tiles * n_tiles + 7) & ~7, held)),
+                       dim3(64 * WN * WM), 0, st, a, m_tiles, n_tiles);
     AMLIKE_HIP(hipGetLastError());
     return AMLIKE_OK;
   });
 }
 
 // Whether 16-byte pieces of x can be copied as they are: rows start on 16 bytes and end on one (or
-// the last piece would bring what lies behind the row), scales on 4.
+// the last piece would bring what lies behind the row), scales on 4; and a tile's 256 rows lie
+// within 32 bits.
 bool Pipeable(const LinearArgs &a, int kind) {
   const int es = IsMx8(kind) ? 1 : 2;
-  return (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.ldx | (uintptr_t)a.k * es) % 16 == 0 &&
+  return a.ldx <= 1 << 22 && (!IsMx8(kind) || a.ld_xs <= 1 << 22) &&
+         (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.ldx | (uintptr_t)a.k * es) % 16 == 0 &&
          (!IsMx8(kind) || (reinterpret_cast<uintptr_t>(a.x_scales) | (uintptr_t)a.ld_xs) % 4 == 0);
 }
 
-template <int TYPE>
+template <int KIND>
 int LaunchLinear(const LinearArgs &args, hipStream_t st) {
-  if (Pipeable(args, TYPE)) {
-    const char *v = getenv("AMLIKE_LIN");
-    const int c = v ? atoi(v) : args.rows >= 2048 ? 1 : 2;
-    if (c == 1) return LaunchPipe<TYPE, 4, 2, 8>(args, st);
-    if (c == 2) return LaunchPipe<TYPE, 2, 2, 4>(args, st);
+  if (Pipeable(args, KIND)) {
+    // 256 x 256 tiles, one block a compute unit, against 128 x 128, two: a unit's two smaller tiles
+    // hold half the work and take .58 of the time (35554 x 2000 x 8600 bf16: 1277 us against 1471).
+    // (With widened 8-bit operands the larger tile's registers do not suffice.)
+    const int64_t units = std::max(1, NumComputeUnits());
+    auto turns = [&](int64_t edge, int64_t held) {
+      const int64_t tiles = (args.rows + edge - 1) / edge * ((args.n_pad + edge - 1) / edge);
+      return (tiles + held - 1) / held;
+    };
+    if constexpr (KIND != kMx8Exact)
+      if (turns(256, units) * 100 <= turns(128, 2 * units) * 58) return LaunchPipe<KIND, 4, 2, 8>(args, st);
+    if (args.rows > 64) return LaunchPipe<KIND, 2, 2, 4>(args, st);
   }
   return ByRows(args, [&](const LinearArgs &a) -> int {
     const int64_t tiles = ((int64_t)a.rows + 63) / 64 * (a.n_pad / 64);
-    hipLaunchKernelGGL(linear_tile_kernel<TYPE>, dim3((unsigned)tiles), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(linear_tile_kernel<KIND>, dim3((unsigned)tiles), dim3(256), 0, st, a);
     AMLIKE_HIP(hipGetLastError());
     return AMLIKE_OK;
   });
