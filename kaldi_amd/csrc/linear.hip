@@ -46,8 +46,9 @@ __global__ __launch_bounds__(256) void linear_pack_scales_kernel(const uint8_t *
                                                                  int64_t words, uint32_t *__restrict__ dst) {
   const int groups = (k + 31) >> 5;
   for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < words; p += (int64_t)gridDim.x * 256) {
-    const int kt = (int)(p / n_pad), row = (int)(p - (int64_t)kt * n_pad);
-    dst[p] = row < n ? load_scales(src + (int64_t)row * groups, kt, groups) : 0x7f7f7f7fu;
+    const int64_t line = p >> 2;
+    const int four = (int)(line / n_pad), row = (int)(line - (int64_t)four * n_pad);
+    dst[p] = row < n ? load_scales(src + (int64_t)row * groups, four * 4 + (int)(p & 3), groups) : 0x7f7f7f7fu;
   }
 }
 
@@ -96,7 +97,7 @@ int PackWeights(amlike_linear *h, const float *weights, int64_t ld, const float 
                        reinterpret_cast<u32x4 *>(h->d_w), static_cast<int *>(flag.ptr));
     AMLIKE_HIP(hipGetLastError());
     if (h->type == AMLIKE_MX8) {
-      const int64_t words = (int64_t)h->k_tiles * h->n_pad;
+      const int64_t words = (int64_t)((h->k_tiles + 3) & ~3) * h->n_pad;
       AMLIKE_HIP(hipMalloc(reinterpret_cast<void **>(&h->d_scales), (size_t)words * 4));
       hipLaunchKernelGGL(linear_pack_scales_kernel, dim3((unsigned)std::min<int64_t>((words + 255) / 256, 1 << 16)), dim3(256), 0,
                          h->stream, static_cast<const uint8_t *>(scales.ptr), h->n, h->k, h->n_pad, words, h->d_scales);

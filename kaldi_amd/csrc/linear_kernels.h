@@ -16,7 +16,7 @@
 // an fp32 one.  For an fp32 output the 8-bit operands are therefore widened to bf16, which holds
 // value times scale exactly, and multiplied there (kMx8Exact), at half the matrix rate.
 //   W:      [k-tile][row, padded to 64][128 bytes], zeros behind both ends
-//   scales: [k-tile][row, padded to 64][4 bytes], 2^0 behind both ends  (8 bits only)
+//   scales: [k-tile / 4][row, padded to 64][k-tile % 4][4 bytes], 2^0 behind both ends  (8 bits only)
 //
 // This header holds the kernels and the choice between them; each kind of product is compiled in a file
 // of its own (linear_bf16.hip ...), the host side is linear.hip.
@@ -423,100 +423,27 @@ __device__ __forceinline__ void finish_wave(const LinearArgs &a, int64_t m, int 
 // vary, and in each case bits 1-3 of the turn take all values.
 __device__ __forceinline__ int turn_x(int r) { return r >> 1 & 7; }
 __device__ __forceinline__ int turn_w(int r) { return (r >> 1 & 7) ^ (r >> 3 & 6); }
-__device__ __forceinline__ int lds_piece(int r, int c) { return r * kChunks + (c ^ turn_x(r)); }
-__device__ __forceinline__ int lds_piece_w(int r, int c) { return r * kChunks + (c ^ turn_w(r)); }
-
-// ---- the plain tile kernel: any size, alignment and type ----------------------------------------------
-// 64 x 64 outputs per block of four waves (32 x 32 each); k-tiles go through registers into LDS.
-template <int TYPE>
-__global__ __launch_bounds__(256) void linear_tile_kernel(LinearArgs a) {
-  __shared__ u32x4 s_w[64 * kChunks], s_x[64 * kChunks];
-  __shared__ uint32_t s_ws[64], s_xs[64];
-  __shared__ float s_c[64][68];
-  constexpr bool kMx = IsMx8(TYPE);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wn = (wave & 1) * 32, wm = (wave >> 1) * 32, r16 = lane & 15, g = lane >> 4;
-  const int n_tiles = a.n_pad >> 6;
-  const int n0 = (int)(blockIdx.x % n_tiles) * 64;
-  const int64_t m0 = (int64_t)(blockIdx.x / n_tiles) * 64;
-  const int bytes = a.k * (kMx ? 1 : 2), groups = (a.k + 31) >> 5;
-  f32x4v acc[2][2] = {};
-  for (int kt = 0; kt < a.k_tiles; ++kt) {
-    u32x4 qw[2], qx[2];
-    uint32_t sc = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int p = tid + i * 256, r = p >> 3, c = p & 7;
-      qw[i] = *reinterpret_cast<const u32x4 *>(a.w + ((int64_t)kt * a.n_pad + n0 + r) * kTileBytes + c * 16);
-      const int64_t m = min(m0 + r, (int64_t)a.rows - 1);
-      qx[i] = load_chunk(a.x + m * a.ldx, kt * kTileBytes + c * 16, bytes);
-    }
-    if constexpr (kMx) {
-      if (tid < 64) sc = a.w_scales[(int64_t)kt * a.n_pad + n0 + tid];
-      else if (tid < 128) sc = load_scales(a.x_scales + min(m0 + tid - 64, (int64_t)a.rows - 1) * a.ld_xs, kt, groups);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int p = tid + i * 256, r = p >> 3, c = p & 7;
-      s_w[lds_piece(r, c)] = qw[i];
-      s_x[lds_piece(r, c)] = qx[i];
-    }
-    if constexpr (kMx) {
-      if (tid < 64) s_ws[tid] = sc;
-      else if (tid < 128) s_xs[tid - 64] = sc;
-    }
-    __syncthreads();
-    Operand<TYPE> fw[2], fx[2];
-#pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      const int rw = wn + f * 16 + r16, rx = wm + f * 16 + r16;
-      fw[f].set(s_w[lds_piece(rw, g)], s_w[lds_piece(rw, g + 4)], kMx ? s_ws[rw] : 0, g);
-      fx[f].set(s_x[lds_piece(rx, g)], s_x[lds_piece(rx, g + 4)], kMx ? s_xs[rx] : 0, g);
-    }
-#pragma unroll
-    for (int f = 0; f < 2; ++f)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) acc[f][e] = tile_product<TYPE>(fw[f], fx[e], acc[f][e]);
-  }
-  // lane (r16, g): row r16 of fragment e of x, outputs g * 4 .. + 3 of fragment f of W
-#pragma unroll
-  for (int f = 0; f < 2; ++f)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<f32x4v *>(&s_c[wm + e * 16 + r16][wn + f * 16 + g * 4]) = acc[f][e];
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int p = tid + i * 256, m = p >> 3, c = p & 7;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = s_c[m][c * 8 + j];
-    finish8(a, m0 + m, n0 + c * 8, v);
-  }
-}
 
 // ---- the pipelined tile kernel: rows of x that start on 16 bytes ---------------------------------------
 // WN x WM waves, each with 64 outputs x 16 MF rows: 16-byte pieces of the k-tiles go from memory
 // straight into LDS (no registers), those of tile t + 1 while tile t is multiplied.
 
-// Asynchronous copies of 16 (4) bytes per lane: lane l's come from base + offset and go to LDS at
-// `lds` + 16 l (4 l).  Written in assembly so that the compiler, which cannot tell the two halves of the
+// Asynchronous copies of 16 bytes per lane: lane l's come from base + offset and go to LDS at
+// `lds` + 16 l.  Written in assembly so that the compiler, which cannot tell the two halves of the
 // buffer apart, does not make every read of LDS wait for them; they have no result register, and
 // wait_copies ends them.
 __device__ __forceinline__ void copy16_to_lds(const uint8_t *base, uint32_t offset, uint32_t lds) {
 #if __HIP_DEVICE_COMPILE__
+  // (the base is the wave's: said again where the compiler has lost sight of it)
+  const uint64_t u = reinterpret_cast<uint64_t>(base);
+  base = reinterpret_cast<const uint8_t *>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32 |
+                                           (uint32_t)__builtin_amdgcn_readfirstlane((int)u));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 #endif
 }
 __device__ __forceinline__ void copy16_to_lds(const uint8_t *p, uint32_t lds) {  // any address per lane
 #if __HIP_DEVICE_COMPILE__
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
-#endif
-}
-__device__ __forceinline__ void copy4_to_lds(const uint8_t *base, uint32_t offset, uint32_t lds) {
-#if __HIP_DEVICE_COMPILE__
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 #endif
 }
 __device__ __forceinline__ void wait_copies() {
@@ -544,24 +471,33 @@ __device__ __forceinline__ uint32_t lds_address(T *p) {
 // Sixteen zero bytes: where pieces behind a row's end come from.
 static __device__ u32x4 g_zero_piece;
 
-// KS such groups of waves share a tile's k-tiles among them, KS at a time, and add up at the end.
-template <int KIND, int WN, int WM, int MF, int STAGES, int KS>
-__global__ __launch_bounds__(64 * WN * WM * KS, WN * WM * KS > 8 ? 4 : 2) void linear_pipe_kernel(LinearArgs a, int m_tiles, int n_tiles) {
+// Waves a SIMD holds of a form, by its registers.
+template <int KIND, int MF, bool COPY>
+constexpr int kWavesPerSimd = !COPY && MF == 1 && KIND != kMx8Exact ? 4 : 2;
+
+// KS such groups of waves share a tile's k-tiles among them and add up at the end.  COPY: rows of x
+// start and end on 16 bytes; otherwise its pieces go through registers.
+template <int KIND, int WN, int WM, int MF, int STAGES, int KS, bool COPY>
+__global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>)) void linear_pipe_kernel(LinearArgs a, int m_tiles, int n_tiles) {
   constexpr int kWaves = WN * WM, BN = 64 * WN, BM = 16 * MF * WM;
   constexpr bool kMx = IsMx8(KIND);
+  static_assert(COPY || STAGES == 2, "one k-tile in registers");
   constexpr int kPiecesW = BN * kChunks / (64 * kWaves), kPiecesX = BM * kChunks / (64 * kWaves);  // per wave
   static_assert((STAGES & (STAGES - 1)) == 0, "a power of two");
   __shared__ u32x4 s_tiles[KS][STAGES][(BN + BM) * kChunks];
-  __shared__ uint32_t s_scales[KS][STAGES][kMx ? BN + BM : 1];
+  __shared__ u32x4 s_scales[KS][2][kMx ? BN + BM : 1];  // rows of W, then of x: the words of four k-tiles
   static_assert(KS == 1 || 4 * MF * kWaves * 64 * (KS - 1) <= KS * STAGES * (BN + BM) * kChunks, "the groups' sums fit where the tiles were");
   const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ks = all / kWaves, wave = all % kWaves;
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-  const int steps = (a.k_tiles + KS - 1) / KS;  // step s of group ks: k-tile s * KS + ks, if there is one
+  // Step s of group ks: k-tile ks * steps + s, if there is one.  (8 bits: scales come for four k-tiles.)
+  const int steps = kMx && KS > 1 ? ((a.k_tiles + KS - 1) / KS + 3) & ~3 : (a.k_tiles + KS - 1) / KS;
   const int wn = wave % WN, wm = wave / WN;
 
   // Blocks go to the 8 dies in turn; each die takes a run of tiles of its own, which its blocks go
   // through side by side, ordered in bands of 4 row tiles: the 32 tiles that a die works on share
-  // 4 strips of x and 8 of W in its L2.
+  // 4 strips of x and 8 of W in its L2 (35554 x 2000 x 8600 bf16: 1148 us; bands of 2: 1208, of 8:
+  // 1308).  Each band begins at outputs of its own, so that the dies do not all ask the memory for the
+  // same lines of W at once (8192 x 4096 x 16384 mx8: 553 us against 594).
   const int total = m_tiles * n_tiles, die = blockIdx.x & 7, per = total >> 3, more = total & 7;
   const int end = die * per + min(die, more) + per + (die < more ? 1 : 0), stride = gridDim.x >> 3;
   int lin = die * per + min(die, more) + (blockIdx.x >> 3);
@@ -574,70 +510,104 @@ __global__ __launch_bounds__(64 * WN * WM * KS, WN * WM * KS > 8 ? 4 : 2) void l
   // all lie before or all behind the padded end (they are then read from the wave's first tile's, of
   // no output); rows of x behind the last are read as the last.
   constexpr int kRowsW = kPiecesW * 8, kRowsX = kPiecesX * 8;
-  constexpr int kScWaves = (BN + BM) / 64;  // waves' worth of scale words, W's first
-  constexpr int kScPer = (kScWaves + kWaves - 1) / kWaves;
-  static_assert(64 % kRowsW == 0, "a wave's rows of W lie in one 64");
+  static_assert(64 % kRowsW == 0 && (!kMx || (BN + BM) / 64 <= kWaves), "a wave's rows of W lie in one 64; a wave's scales are of 64 rows");
   int64_t m0;
   int n0;
-  const uint8_t *bw, *bx, *bsc[kMx ? kScPer : 1];
-  uint32_t ow[kPiecesW], ox[kPiecesX], osc[kMx ? kScPer : 1];
+  const uint8_t *bw, *bx;
+  uint32_t ow[kPiecesW], ox[kPiecesX];
+  // What comes through registers for a step: pieces of x, scales.  (Asked for and put into LDS in one
+  // turn of the loop: carried into the next, the compiler would wait for it at once.)
+  struct Held {
+    u32x4 x[kPiecesX], scales;
+  };
 #pragma unroll
   for (int i = 0; i < kPiecesW; ++i) {
     const int r = i * 8 + (lane >> 3);
     ow[i] = r * kTileBytes + ((lane & 7) ^ turn_w(wave * kRowsW + r)) * 16;
   }
+  auto last_row = [&]() __attribute__((always_inline)) { return (int)min((int64_t)BM, a.rows - m0) - 1; };
   auto place = [&]() __attribute__((always_inline)) {
     const int band = lin / (4 * n_tiles), in = lin - band * 4 * n_tiles, high = min(4, m_tiles - band * 4);
     m0 = (int64_t)(band * 4 + in % high) * BM;
-    n0 = in / high * BN;
+    int nt = in / high + (int)((int64_t)band * n_tiles / ((m_tiles + 3) >> 2));
+    if (nt >= n_tiles) nt -= n_tiles;
+    n0 = nt * BN;
     const int wrow = n0 + wave * kRowsW;
     bw = a.w + (int64_t)(wrow < a.n_pad ? wrow : 0) * kTileBytes;
     bx = a.x + m0 * a.ldx;
-    const int last = (int)min((int64_t)BM, a.rows - m0) - 1;
 #pragma unroll
     for (int i = 0; i < kPiecesX; ++i) {
       const int r = wave * kRowsX + i * 8 + (lane >> 3);
-      ox[i] = (uint32_t)min(r, last) * (uint32_t)a.ldx + ((lane & 7) ^ turn_x(r)) * 16;
+      ox[i] = (uint32_t)min(r, last_row()) * (uint32_t)a.ldx + (COPY ? ((lane & 7) ^ turn_x(r)) * 16 : 0);
+    }
+  };
+  // Byte of a row at which this lane's piece i of k-tile kt lies.
+  auto piece_at = [&](int i, int kt) __attribute__((always_inline)) {
+    const int r = wave * kRowsX + i * 8 + (lane >> 3);
+    return kt * kTileBytes + ((lane & 7) ^ turn_x(r)) * 16;
+  };
+
+  auto fetch = [&](int step, Held &held) __attribute__((always_inline)) {
+    const int b = step & (STAGES - 1), kt = ks * steps + step;
+    if (KS > 1 && kt >= a.k_tiles) return;
+    const uint32_t lw = lds_address(&s_tiles[ks][b][wave * kPiecesW * 64]), lx = lds_address(&s_tiles[ks][b][BN * kChunks + wave * kPiecesX * 64]);
+    const uint8_t *w = bw + kt * w_step, *x = bx + (COPY ? kt * kTileBytes : 0);
+#pragma unroll
+    for (int i = 0; i < kPiecesW; ++i) copy16_to_lds(w, ow[i], lw + i * 1024);
+    const bool whole = (kt + 1) * kTileBytes <= bytes;  // not the last k-tile, or not a short one
+    if constexpr (COPY) {
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < kPiecesX; ++i) copy16_to_lds(x, ox[i], lx + i * 1024);
+      } else {  // zeros behind the rows' end
+#pragma unroll
+        for (int i = 0; i < kPiecesX; ++i)
+          copy16_to_lds(piece_at(i, kt) < bytes ? x + ox[i] : reinterpret_cast<const uint8_t *>(&g_zero_piece), lx + i * 1024);
+      }
+    } else {
+      typedef u32x4 u32x4_byte __attribute__((aligned(1)));
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < kPiecesX; ++i) held.x[i] = *reinterpret_cast<const u32x4_byte *>(x + ox[i] + piece_at(i, kt));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPiecesX; ++i) held.x[i] = load_chunk(x + ox[i], piece_at(i, kt), bytes);
+      }
     }
     if constexpr (kMx) {
-#pragma unroll
-      for (int i = 0; i < kScPer; ++i) {
-        const int r = (wave + i * kWaves) * 64;  // the wave's first
-        if (r < BN) {
-          bsc[i] = reinterpret_cast<const uint8_t *>(a.w_scales + (n0 + r < a.n_pad ? n0 + r : 0));
-          osc[i] = lane * 4;
+      if ((step & 3) == 0 && wave < (BN + BM) / 64) {  // the scales of this k-tile and the next three
+        const int r = wave * 64;  // the wave's first row
+        const bool of_w = r < BN;
+        const int64_t line = (int64_t)(kt >> 2) * a.n_pad + (n0 + r < a.n_pad ? n0 + r : 0);
+        const uint8_t *base = of_w ? reinterpret_cast<const uint8_t *>(a.w_scales) + line * 16 : a.x_scales + m0 * a.ld_xs + (int64_t)kt * 4;
+        const uint32_t offset = of_w ? lane * 16 : (uint32_t)min(r - BN + lane, last_row()) * (uint32_t)a.ld_xs;
+        if constexpr (COPY) {  // (what a row's last 16 bytes hold behind its last scale is put right on reading)
+          copy16_to_lds(base, offset, lds_address(&s_scales[ks][step >> 2 & 1][r]));
         } else {
-          bsc[i] = a.x_scales + m0 * a.ld_xs;
-          osc[i] = (uint32_t)min(r - BN + lane, last) * (uint32_t)a.ld_xs;
+          typedef u32x4 u32x4_byte __attribute__((aligned(1)));
+          const int groups = (a.k + 31) >> 5;
+          if (of_w || kt * 4 + 16 <= groups) {
+            held.scales = *reinterpret_cast<const u32x4_byte *>(base + offset);
+          } else {
+            u32x4 q = {0, 0, 0, 0};
+#pragma clang loop unroll(disable)
+            for (int i = 0; i < 4; ++i) q = u32x4{q[1], q[2], q[3], load_scales(base - (int64_t)kt * 4 + offset, kt + i, groups)};
+            held.scales = q;
+          }
         }
       }
     }
   };
-
-  auto fetch = [&](int step) __attribute__((always_inline)) {
-    const int b = step & (STAGES - 1), kt = step * KS + ks;
-    if (KS > 1 && kt >= a.k_tiles) return;
-    const uint32_t lw = lds_address(&s_tiles[ks][b][wave * kPiecesW * 64]), lx = lds_address(&s_tiles[ks][b][BN * kChunks + wave * kPiecesX * 64]);
-    const uint8_t *w = bw + kt * w_step, *x = bx + kt * kTileBytes;
+  // What fetch(step) brought into registers goes to LDS.
+  auto put = [&](int step, const Held &held) __attribute__((always_inline)) {
+    if constexpr (!COPY) {
+      if (KS == 1 || ks * steps + step < a.k_tiles) {
 #pragma unroll
-    for (int i = 0; i < kPiecesW; ++i) copy16_to_lds(w, ow[i], lw + i * 1024);
-    if ((kt + 1) * kTileBytes <= bytes) {
-#pragma unroll
-      for (int i = 0; i < kPiecesX; ++i) copy16_to_lds(x, ox[i], lx + i * 1024);
-    } else {  // the last k-tile, short: zeros behind the rows' end
-#pragma unroll
-      for (int i = 0; i < kPiecesX; ++i) {
-        const int r = wave * kRowsX + i * 8 + (lane >> 3), at = kt * kTileBytes + ((lane & 7) ^ turn_x(r)) * 16;
-        copy16_to_lds(at < bytes ? x + ox[i] : reinterpret_cast<const uint8_t *>(&g_zero_piece), lx + i * 1024);
+        for (int i = 0; i < kPiecesX; ++i) s_tiles[ks][step & 1][BN * kChunks + (wave * kPiecesX + i) * 64 + lane] = held.x[i];
       }
     }
-    if constexpr (kMx) {
-#pragma unroll
-      for (int i = 0; i < kScPer; ++i) {
-        const int q = wave + i * kWaves;
-        if (q < kScWaves) copy4_to_lds(bsc[i] + (int64_t)kt * (q < BN / 64 ? a.n_pad * 4 : 4), osc[i], lds_address(&s_scales[ks][b][q * 64]));
-      }
-    }
+    if constexpr (kMx && !COPY)
+      if ((step & 3) == 0 && wave < (BN + BM) / 64) s_scales[ks][step >> 2 & 1][wave * 64 + lane] = held.scales;
   };
 
   const int ch = KIND == kMx8Exact || a.out_type == AMLIKE_F32 ? 4 : a.out_type == AMLIKE_MX8 ? 16 : 8;
@@ -646,14 +616,19 @@ __global__ __launch_bounds__(64 * WN * WM * KS, WN * WM * KS > 8 ? 4 : 2) void l
   for (int f = 0; f < 4; ++f) row_w[f] = wn * 64 + fragment_output(ch, f, r16);
 
   // k-tiles of a tile that start() asks for: with two buffers both, with more all but the one that the
-  // first turn of the loop asks for.
-  constexpr int kAhead = STAGES == 2 ? 2 : STAGES - 1;
+  // first turn of the loop asks for, through registers one.
+  constexpr int kAhead = !COPY ? 1 : STAGES == 2 ? 2 : STAGES - 1;
   // A tile's first k-tiles and its biases, on their way while the tile before is stored.  The memory
   // unit answers in order: when the biases are there, so are the k-tiles.
   f32x4v bias[4];
+  Held first;  // step 0's
   auto start = [&]() __attribute__((always_inline)) {
     place();
-    for (int s = 0; s < min(kAhead, steps); ++s) fetch(s);
+    fetch(0, first);
+    for (int s = 1; s < min(kAhead, steps); ++s) {
+      Held none;  // (copies only: x, and scales with step 0's)
+      fetch(s, none);
+    }
     const int n = n0 + wn * 64;
     if (ch == 4) load_bias<4>(a, n, g, bias);
     else if (ch == 16) load_bias<16>(a, n, g, bias);
@@ -671,10 +646,24 @@ __global__ __launch_bounds__(64 * WN * WM * KS, WN * WM * KS > 8 ? 4 : 2) void l
 #pragma unroll
       for (int e = 0; e < MF; ++e) acc[f][e] = ks == 0 ? bias[f] : f32x4v{0, 0, 0, 0};
     }
+    auto operand = [&](int step, const u32x4 *tile, int first, int row, int turn) __attribute__((always_inline)) {
+      Operand<KIND> o;
+      uint32_t sc = 0;
+      if constexpr (kMx) {
+        sc = reinterpret_cast<const uint32_t *>(&s_scales[ks][step >> 2 & 1][first + row])[step & 3];
+        if constexpr (COPY) {  // 2^0 behind the row's last scale
+          const int groups = ((a.k + 31) >> 5) - (ks * steps + step) * 4;
+          if (groups < 4) sc = (sc & ~(~0u << (8 * groups))) | (0x7f7f7f7fu << (8 * groups));
+        }
+      }
+      o.set(tile[row * kChunks + (g ^ turn)], tile[row * kChunks + (g ^ 4 ^ turn)], sc, g);
+      return o;
+    };
     int step = 0;
 #if __HIP_DEVICE_COMPILE__
     asm volatile("" : "+s"(step));  // (one copy of the loop's body: the first steps are not to be peeled off)
 #endif
+    put(0, first);
 #pragma clang loop unroll(disable)
     for (; step < steps; ++step) {
       // This wave's pieces for the step have to be in LDS, and its reads of the step before done.  The
@@ -683,31 +672,23 @@ __global__ __launch_bounds__(64 * WN * WM * KS, WN * WM * KS > 8 ? 4 : 2) void l
       else if (STAGES == 2 || step + STAGES - 1 >= steps) wait_copies();
       else wait_copies_but<(STAGES - 2) * (kPiecesW + kPiecesX)>();
       __builtin_amdgcn_s_barrier();  // everybody's
-      if (STAGES == 2 ? step >= 1 && step + 1 < steps : step + STAGES - 1 < steps) fetch(step + STAGES - 1);
-      const int b = step & (STAGES - 1), kt = step * KS + ks;
-      if (KS > 1 && kt >= a.k_tiles) continue;
-      const int groups = kMx ? min(4, ((a.k + 31) >> 5) - kt * 4) : 0;
+      Held held;
+      const bool ahead = step + STAGES - 1 >= kAhead && step + STAGES - 1 < steps;
+      if (ahead) fetch(step + STAGES - 1, held);
+      const int b = step & (STAGES - 1);
+      if (KS == 1 || ks * steps + step < a.k_tiles) {
       const u32x4 *tw = s_tiles[ks][b], *tx = tw + BN * kChunks;
-      const uint32_t *sw = s_scales[ks][b], *sx = sw + (kMx ? BN : 0);
-      auto operand = [&](const u32x4 *tile, const uint32_t *scales, int row, int turn) __attribute__((always_inline)) {
-        Operand<KIND> o;
-        uint32_t sc = 0;
-        if constexpr (kMx) {
-          sc = scales[row];
-          if (groups < 4) sc = (sc & ~(~0u << (8 * groups))) | (0x7f7f7f7fu << (8 * groups));  // what lies behind the row's scales
-        }
-        o.set(tile[row * kChunks + (g ^ turn)], tile[row * kChunks + (g ^ 4 ^ turn)], sc, g);
-        return o;
-      };
       Operand<KIND> fw[4];
 #pragma unroll
-      for (int f = 0; f < 4; ++f) fw[f] = operand(tw, sw, row_w[f], turn_w(row_w[f]));
+      for (int f = 0; f < 4; ++f) fw[f] = operand(step, tw, 0, row_w[f], turn_w(row_w[f]));
 #pragma unroll
       for (int e = 0; e < MF; ++e) {
-        const Operand<KIND> fx = operand(tx, sx, wm * 16 * MF + e * 16 + r16, turn_x(r16));
+        const Operand<KIND> fx = operand(step, tx, BN, wm * 16 * MF + e * 16 + r16, turn_x(r16));
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[f][e] = tile_product<KIND>(fw[f], fx, acc[f][e]);
       }
+      }
+      if (ahead) put(step + STAGES - 1, held);  // (where nobody reads now: the barriers of this turn and the next)
     }
     const int64_t m = m0 + wm * 16 * MF;
     const int n = n0 + wn * 64;
@@ -787,7 +768,7 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
       for (int f = 0; f < NT; ++f) {
         qw[u][f][0] = *reinterpret_cast<const u32x4 *>(p + f * 16 * kTileBytes);
         qw[u][f][1] = *reinterpret_cast<const u32x4 *>(p + f * 16 * kTileBytes + 64);
-        sw[u][f] = kMx ? a.w_scales[(int64_t)kt * a.n_pad + n0 + f * 16 + r16] : 0;
+        sw[u][f] = kMx ? a.w_scales[((int64_t)(kt >> 2) * a.n_pad + n0 + f * 16 + r16) * 4 + (kt & 3)] : 0;
       }
       const int at = kt * kTileBytes + g * 16;
       if ((kt + 1) * kTileBytes <= bytes) {
@@ -868,28 +849,25 @@ int ByRows(LinearArgs a, F launch) {
   return AMLIKE_OK;
 }
 
-template <int KIND, int WN, int WM, int MF, int STAGES, int KS>
+template <int KIND, int WN, int WM, int MF, int STAGES, int KS, bool COPY = true>
 int LaunchPipe(const LinearArgs &args, hipStream_t st) {
   return ByRows(args, [&](const LinearArgs &a) -> int {
     const int m_tiles = (a.rows + 16 * MF * WM - 1) / (16 * MF * WM), n_tiles = (a.n_pad + 64 * WN - 1) / (64 * WN);
-    // as many blocks as the device holds at once, by waves (8 a compute unit) and LDS, in eights
-    constexpr int kLds = KS * STAGES * (64 * WN + 16 * MF * WM) * (kTileBytes + (IsMx8(KIND) ? 4 : 0)) + 16;
-    const int held = std::max(8, NumComputeUnits() * std::min(std::max(1, 8 / (WN * WM * KS)), 163840 / kLds) & ~7);
-    hipLaunchKernelGGL((linear_pipe_kernel<KIND, WN, WM, MF, STAGES, KS>), dim3((unsigned)std::min((m_tiles * n_tiles + 7) & ~7, held)),
+    // as many blocks as the device holds at once, by waves and LDS, in eights
+    constexpr int kLds = KS * (64 * WN + 16 * MF * WM) * (STAGES * kTileBytes + (IsMx8(KIND) ? 32 : 0)) + 64;
+    const int held = std::max(8, NumComputeUnits() * std::min(4 * kWavesPerSimd<KIND, MF, COPY> / (WN * WM * KS), 163840 / kLds) & ~7);
+    hipLaunchKernelGGL((linear_pipe_kernel<KIND, WN, WM, MF, STAGES, KS, COPY>), dim3((unsigned)std::min((m_tiles * n_tiles + 7) & ~7, held)),
                        dim3(64 * WN * WM * KS), 0, st, a, m_tiles, n_tiles);
     AMLIKE_HIP(hipGetLastError());
     return AMLIKE_OK;
   });
 }
 
-// Whether 16-byte pieces of x can be copied as they are: rows start on 16 bytes and end on one (or
-// the last piece would bring what lies behind the row), scales on 4; and a tile's 256 rows lie
-// within 32 bits.
-bool Pipeable(const LinearArgs &a, int kind) {
-  const int es = IsMx8(kind) ? 1 : 2;
-  return a.ldx <= 1 << 22 && (!IsMx8(kind) || a.ld_xs <= 1 << 22) &&
-         (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.ldx | (uintptr_t)a.k * es) % 16 == 0 &&
-         (!IsMx8(kind) || (reinterpret_cast<uintptr_t>(a.x_scales) | (uintptr_t)a.ld_xs) % 4 == 0);
+// Whether 16-byte pieces of x can be copied as they are: rows, of scales too, start on 16 bytes and
+// end on one (or the last piece would bring what lies behind the row; scales are looked after).
+bool Copyable(const LinearArgs &a, int kind) {
+  return (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.ldx | (uintptr_t)a.k * (IsMx8(kind) ? 1 : 2)) % 16 == 0 &&
+         (!IsMx8(kind) || (reinterpret_cast<uintptr_t>(a.x_scales) | (uintptr_t)a.ld_xs) % 16 == 0);
 }
 
 template <int KIND, int NT, int MT>
@@ -897,16 +875,6 @@ int LaunchThin(const LinearArgs &args, hipStream_t st) {
   return ByRows(args, [&](const LinearArgs &a) -> int {
     const int m_tiles = (a.rows + 16 * MT - 1) / (16 * MT);
     hipLaunchKernelGGL((linear_thin_kernel<KIND, NT, MT>), dim3((unsigned)m_tiles * (a.n_pad / (16 * NT))), dim3(512), 0, st, a, m_tiles);
-    AMLIKE_HIP(hipGetLastError());
-    return AMLIKE_OK;
-  });
-}
-
-template <int KIND>
-int LaunchTile(const LinearArgs &args, hipStream_t st) {
-  return ByRows(args, [&](const LinearArgs &a) -> int {
-    const int64_t tiles = ((int64_t)a.rows + 63) / 64 * (a.n_pad / 64);
-    hipLaunchKernelGGL(linear_tile_kernel<KIND>, dim3((unsigned)tiles), dim3(256), 0, st, a);
     AMLIKE_HIP(hipGetLastError());
     return AMLIKE_OK;
   });
@@ -937,7 +905,7 @@ int LaunchLinear(const LinearArgs &a, hipStream_t st) {
     if (a.rows <= 16) return wide ? LaunchThin<KIND, 2, 1>(a, st) : LaunchThin<KIND, 1, 1>(a, st);
     return wide ? LaunchThin<KIND, 2, 2>(a, st) : LaunchThin<KIND, 1, 2>(a, st);
   }
-  if (!Pipeable(a, KIND)) return a.rows <= 64 ? LaunchThin<KIND, 2, 4>(a, st) : LaunchTile<KIND>(a, st);
+  if (a.ldx > 1 << 22 || a.ld_xs > 1 << 22) return LaunchThin<KIND, 2, 4>(a, st);  // a tile's rows have to lie within 32 bits
   const double units = std::max(1, NumComputeUnits()), kt = a.k_tiles;
   auto turns = [&](int edge) {
     return std::ceil((double)(((int64_t)a.rows + edge - 1) / edge * ((a.n_pad + edge - 1) / edge)) / units);
@@ -945,6 +913,10 @@ int LaunchLinear(const LinearArgs &a, hipStream_t st) {
   const double t256 = turns(256), t128 = turns(128), t64 = turns(64);
   const double cost[5] = {t256 * (1.62 * kt + 7), t128 <= 1 ? 0.65 * kt + 2 : std::ceil(t128 / 2) * (0.95 * kt + 4), t128 * (0.55 * kt + 3),
                           t64 <= 1 ? 0.31 * kt + 1 : std::ceil(t64 / 2) * (0.38 * kt + 2), t64 * (0.24 * kt + 2)};
+  if (!Copyable(a, KIND))
+    return std::ceil(t64 / 4) * std::min(t64, 4.0) * 0.36 < (t128 <= 1 ? 1.25 : std::ceil(t128 / 2) * 2.0)
+               ? LaunchPipe<KIND, 1, 4, 1, 2, 1, false>(a, st)
+               : LaunchPipe<KIND, 2, 2, 4, 2, 1, false>(a, st);
   // (with widened 8-bit operands the largest tile's registers do not suffice)
   const int first = KIND == kMx8Exact ? 1 : 0, best = (int)(std::min_element(cost + first, cost + 5) - cost);
   if (best == 1) return LaunchPipe<KIND, 2, 2, 4, 2, 1>(a, st);
