@@ -259,7 +259,8 @@ enum amlike_type {
  * data[r * ld + c]; data is aligned to its element.  AMLIKE_MX8: data are bytes, and the scale
  * of (r, c) is scales[r * ld_scales + c / 32].  Any ld >= the columns, any ld_scales >=
  * ceil(columns / 32); what lies behind a row's columns and behind the last row is neither
- * needed nor written.  Rows that start on 16 bytes (and MX8 scales on 4) are the fast case. */
+ * needed nor written.  Rows (of scales too) that start on 16 bytes, and for amlike_linear's x hold a
+ * multiple of 16 bytes, are the fast case. */
 typedef struct amlike_matrix {
   void *data;
   void *scales; /* AMLIKE_MX8 only, else NULL */

@@ -3,10 +3,10 @@
 // (amlike_linear_*).
 //
 // Layout.  A k-tile is 128 bytes of a row: 64 columns in 16 bits, 128 in 8.  Both kinds of matrix
-// instruction used (16x16x32 bf16 / f16, 16x16x128 scaled e4m3) then look alike: lane l of a
-// fragment holds row l % 16 and, of its k-tile, the 32 bytes l / 16 -- the 16-bit ones as two
-// instructions of 16 bytes each (which columns meet in one instruction does not matter as long as
-// both operands agree), the 8-bit one as a single instruction whose scale is that lane's byte.
+// instruction used (16x16x32 bf16 / f16, 16x16x128 scaled e4m3) then look alike: with g = l / 16,
+// lane l of a fragment holds row l % 16 and, of its k-tile, the 16-byte pieces g and g + 4 -- as
+// two 16-bit instructions of one piece each, or as a single 8-bit one, whose scale operand is that
+// of the columns 32 g .. 32 g + 31 (a lane's scale is not that of its own values).
 // W is the instructions' first operand and x the second, so that a lane's results are 4 outputs of
 // one row of x per fragment.
 // The 8-bit instruction aligns the products of a few neighbouring columns to the largest of them
@@ -424,9 +424,17 @@ __device__ __forceinline__ void finish_wave(const LinearArgs &a, int64_t m, int 
 __device__ __forceinline__ int turn_x(int r) { return r >> 1 & 7; }
 __device__ __forceinline__ int turn_w(int r) { return (r >> 1 & 7) ^ (r >> 3 & 6); }
 
-// ---- the pipelined tile kernel: rows of x that start on 16 bytes ---------------------------------------
+// ---- the pipelined tile kernel ---------------------------------------------------------------------------
 // WN x WM waves, each with 64 outputs x 16 MF rows: 16-byte pieces of the k-tiles go from memory
-// straight into LDS (no registers), those of tile t + 1 while tile t is multiplied.
+// straight into LDS (no registers), those of later tiles while one is multiplied; blocks stay and go
+// from tile to tile.
+// What bounds the 256 x 256 form (8192 x 4096 x 16384): in bf16 852 us, 1.29 PFLOP/s, the library's plain
+// product 808; the matrix pipe is busy for .59 of the cycles, at the clock the chip holds under
+// such operands.  In mx8 545-560 us, 2.0 PFLOP/s (library, one scale for all: 438): without the copies it
+// takes 461, without the matrix instructions 466, without the epilogue 501, so copies and products
+// hide each other only in part: 64 KB have to come within the time of one k-tile's products, and LDS
+// has no room for a third buffer.  (Tried, and no faster: waves of a SIMD reading and multiplying
+// in turns, four waves of 128 x 128, touching the lines ahead.)
 
 // Asynchronous copies of 16 bytes per lane: lane l's come from base + offset and go to LDS at
 // `lds` + 16 l.  Written in assembly so that the compiler, which cannot tell the two halves of the
@@ -830,11 +838,11 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
 
 namespace {
 
-// Calls `launch` on stretches of the rows, all of them but for outputs beyond 2^35 elements: a grid
-// holds less than 2^32 threads, 2^24 blocks of 256.
+// Calls `launch` on stretches of the rows, all of them but for outputs beyond 2^33 elements: a grid
+// holds less than 2^32 threads, 2^23 blocks of 512.
 template <typename F>
 int ByRows(LinearArgs a, F launch) {
-  const int64_t most = std::max<int64_t>(((int64_t)1 << 35) / a.n_pad / 256 * 256, 256);
+  const int64_t most = std::max<int64_t>(((int64_t)1 << 33) / a.n_pad / 256 * 256, 256);
   const int64_t rows = a.rows;
   const int rb = a.res_type < 0 ? 0 : TypeBytes(a.res_type), ob = TypeBytes(a.out_type);
   for (int64_t r = 0; r < rows; r += most) {
@@ -886,9 +894,9 @@ int LaunchThin(const LinearArgs &args, hipStream_t st) {
 // pipelined kernel of 64 x 64 takes 18.0 us for 64 x 4096 x 4096 bf16, the thin one 24.4; at 32 rows
 // of mx8 13.1 and 9.7.
 //
-// More rows, where the pipelined kernel can read them: the form with the least estimated time, from
-// the turns that the busiest compute unit has to take.  Microseconds per k-tile and per turn,
-// measured in bf16 at the sizes behind each line; only their relation matters.
+// More rows: the form of the pipelined kernel with the least estimated time, from the turns that the
+// busiest compute unit has to take.  Microseconds per k-tile and per turn, measured in bf16 at the
+// sizes behind each line; only their relation matters.
 //   256 x 256, 8 waves                      1.62 kt + 7    35554 x 2000 x 8600: 1118 (measured 1157)
 //   128 x 128, 4 waves, alone on its unit   0.65 kt + 2    1024 x 4096 x 4096: 44 (44.5)
 //              two of them                  0.95 kt + 4    4096 x 2048 x 2048: 34 (34.4)
@@ -896,6 +904,9 @@ int LaunchThin(const LinearArgs &args, hipStream_t st) {
 //   64 x 64, 4 waves, alone                 0.31 kt + 1    300 x 360 x 2000: 5.9 (5.5, launch and all)
 //            two of them                    0.38 kt + 2    1024 x 4096 x 4096: 53 (54)
 //   64 x 64, 2 groups of 4 waves            0.24 kt + 2    256 x 4096 x 4096: 17 (18.3)
+// Rows of x that do not start and end on 16 bytes go through registers, in two forms:
+//   64 x 64, four blocks a unit             0.36 kt each   1237 x 1999 x 2001 bf16: 30.0 (128 x 128: 39.5)
+//   128 x 128, alone / two of them   1.25 kt / 2.0 kt      2000 x 2002 x 4096 mx8: 32.0 (64 x 64: 53.1)
 }  // namespace
 
 template <int KIND>

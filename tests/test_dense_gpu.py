@@ -208,7 +208,7 @@ def linear_error(k, mass, pre, act_y, y, tout, act, type_="bf16"):
 
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 2048, 200), (2, 33, 5), (3, 360, 129), (7, 129, 64), (16, 512, 320), (17, 250, 96), (31, 1000, 65),
          (33, 127, 257), (64, 128, 128), (65, 63, 191), (100, 360, 300), (129, 200, 70), (300, 96, 264), (257, 520, 513), (640, 136, 520),
-         (2100, 80, 8200), (4099, 72, 4160)]
+         (2100, 80, 8200), (4099, 72, 4160), (9000, 65, 520)]
 
 
 @pytest.mark.parametrize("type_", ["bf16", "f16", "mx8"])
