@@ -423,6 +423,10 @@ __device__ __forceinline__ void finish_wave(const LinearArgs &a, int64_t m, int 
 // vary, and in each case bits 1-3 of the turn take all values.
 __device__ __forceinline__ int turn_x(int r) { return r >> 1 & 7; }
 __device__ __forceinline__ int turn_w(int r) { return (r >> 1 & 7) ^ (r >> 3 & 6); }
+// The scales of four k-tiles are 16 bytes per row.  Those of row r of W lie at place scale_place(r), each
+// 16 rows turned by 4 against the 16 before, for the same reason; row_at_place is its inverse.
+__device__ __forceinline__ int scale_place(int r) { return (r & ~15) | ((r + (r >> 4 << 2)) & 15); }
+__device__ __forceinline__ int row_at_place(int l) { return (l & ~15) | ((l - (l >> 4 << 2)) & 15); }
 
 // ---- the pipelined tile kernel ---------------------------------------------------------------------------
 // WN x WM waves, each with 64 outputs x 16 MF rows: 16-byte pieces of the k-tiles go from memory
@@ -588,7 +592,7 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
         const bool of_w = r < BN;
         const int64_t line = (int64_t)(kt >> 2) * a.n_pad + (n0 + r < a.n_pad ? n0 + r : 0);
         const uint8_t *base = of_w ? reinterpret_cast<const uint8_t *>(a.w_scales) + line * 16 : a.x_scales + m0 * a.ld_xs + (int64_t)kt * 4;
-        const uint32_t offset = of_w ? lane * 16 : (uint32_t)min(r - BN + lane, last_row()) * (uint32_t)a.ld_xs;
+        const uint32_t offset = of_w ? row_at_place(lane) * 16 : (uint32_t)min(r - BN + lane, last_row()) * (uint32_t)a.ld_xs;
         if constexpr (COPY) {  // (what a row's last 16 bytes hold behind its last scale is put right on reading)
           copy16_to_lds(base, offset, lds_address(&s_scales[ks][step >> 2 & 1][r]));
         } else {
@@ -654,11 +658,11 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
 #pragma unroll
       for (int e = 0; e < MF; ++e) acc[f][e] = ks == 0 ? bias[f] : f32x4v{0, 0, 0, 0};
     }
-    auto operand = [&](int step, const u32x4 *tile, int first, int row, int turn) __attribute__((always_inline)) {
+    auto operand = [&](int step, const u32x4 *tile, int row, int turn, int scale_row) __attribute__((always_inline)) {
       Operand<KIND> o;
       uint32_t sc = 0;
       if constexpr (kMx) {
-        sc = reinterpret_cast<const uint32_t *>(&s_scales[ks][step >> 2 & 1][first + row])[step & 3];
+        sc = reinterpret_cast<const uint32_t *>(&s_scales[ks][step >> 2 & 1][scale_row])[step & 3];
         if constexpr (COPY) {  // 2^0 behind the row's last scale
           const int groups = ((a.k + 31) >> 5) - (ks * steps + step) * 4;
           if (groups < 4) sc = (sc & ~(~0u << (8 * groups))) | (0x7f7f7f7fu << (8 * groups));
@@ -688,10 +692,10 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
       const u32x4 *tw = s_tiles[ks][b], *tx = tw + BN * kChunks;
       Operand<KIND> fw[4];
 #pragma unroll
-      for (int f = 0; f < 4; ++f) fw[f] = operand(step, tw, 0, row_w[f], turn_w(row_w[f]));
+      for (int f = 0; f < 4; ++f) fw[f] = operand(step, tw, row_w[f], turn_w(row_w[f]), scale_place(row_w[f]));
 #pragma unroll
       for (int e = 0; e < MF; ++e) {
-        const Operand<KIND> fx = operand(step, tx, BN, wm * 16 * MF + e * 16 + r16, turn_x(r16));
+        const Operand<KIND> fx = operand(step, tx, wm * 16 * MF + e * 16 + r16, turn_x(r16), BN + wm * 16 * MF + e * 16 + r16);
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[f][e] = tile_product<KIND>(fw[f], fx, acc[f][e]);
       }
