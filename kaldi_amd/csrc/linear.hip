@@ -254,7 +254,7 @@ int amlike_linear_apply(amlike_linear_t *h, const float *x, int32_t ld, int32_t 
   if (rows == 0) return AMLIKE_OK;
   std::lock_guard<std::mutex> lock(h->mu);
   const size_t xrow = (size_t)h->k * sizeof(float), orow = (size_t)h->n * sizeof(float);
-  const int groups = (h->k + 31) / 32;
+  const int groups = ((h->k + 31) / 32 + 15) / 16 * 16;  // (a row's scales start on 16 bytes)
   const size_t ldq = ((size_t)h->k + 15) / 16 * 16, values = ldq * TypeBytes(h->type) * rows;
   int rc = h->ws_x.Reserve(xrow * rows);
   if (rc == AMLIKE_OK) rc = h->ws_q.Reserve(values + (h->type == AMLIKE_MX8 ? (size_t)groups * rows : 0));

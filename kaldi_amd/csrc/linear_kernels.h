@@ -680,9 +680,10 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
     for (; step < steps; ++step) {
       // This wave's pieces for the step have to be in LDS, and its reads of the step before done.  The
       // copies of the STAGES - 2 steps behind may be under way (in order: nothing else is behind them).
+      const int behind = step + STAGES - 2;  // the last of them, if it was asked for (a group's last steps may have no k-tile)
       if (step < kAhead) wait_lds();
-      else if (STAGES == 2 || step + STAGES - 1 >= steps) wait_copies();
-      else wait_copies_but<(STAGES - 2) * (kPiecesW + kPiecesX)>();
+      else if (STAGES > 2 && behind < steps && ks * steps + behind < a.k_tiles) wait_copies_but<(STAGES - 2) * (kPiecesW + kPiecesX)>();
+      else wait_copies();
       __builtin_amdgcn_s_barrier();  // everybody's
       Held held;
       const bool ahead = step + STAGES - 1 >= kAhead && step + STAGES - 1 < steps;

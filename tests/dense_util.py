@@ -64,7 +64,8 @@ class DeviceMatrix:
         self.buf = raw.view(dt)[offset:].view(rows + behind, self.ld)
         self.scales = None
         if type_ == "mx8":
-            self.ld_scales = (cols + 31) // 32 + (pad and 1)
+            # (rows of scales that start on 16 bytes where those of values may, and any others)
+            self.ld_scales = ((cols + 31) // 32 + 15) // 16 * 16 if pad % 8 == 0 else (cols + 31) // 32 + 1
             self.scales = torch.full((rows + behind, self.ld_scales), 0xFF, dtype=torch.uint8, device="cuda")
         if fill is not None:
             if type_ == "mx8":

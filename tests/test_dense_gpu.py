@@ -58,7 +58,7 @@ def test_convert_to_mx8_borders(amlike_device):
     dense.ConvertDevice(dx.m, len(rows), 32, out.m)
     torch.cuda.synchronize()
     q, s = U.to_mx8(x)
-    assert torch.equal(out.scales[:len(rows)].cpu(), s)
+    assert torch.equal(out.scales[:len(rows), :1].cpu(), s)
     want = U.from_mx8(q, s)
     assert torch.equal(torch.isnan(want), ~torch.isfinite(x)) and U.same(out.values(), want)
 
@@ -208,14 +208,15 @@ def linear_error(k, mass, pre, act_y, y, tout, act, type_="bf16"):
 
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 2048, 200), (2, 33, 5), (3, 360, 129), (7, 129, 64), (16, 512, 320), (17, 250, 96), (31, 1000, 65),
          (33, 127, 257), (64, 128, 128), (65, 63, 191), (100, 360, 300), (129, 200, 70), (300, 96, 264), (257, 520, 513), (640, 136, 520),
-         (2100, 80, 8200), (4099, 72, 4160), (9000, 65, 520)]
+         (2100, 80, 8200), (4099, 72, 4160), (9000, 65, 520),
+         (256, 3328, 4096), (200, 1984, 1032)]
 
 
 @pytest.mark.parametrize("type_", ["bf16", "f16", "mx8"])
 @pytest.mark.parametrize("rows,k,n", SIZES)
 def test_linear_is_exact_on_small_integers(amlike_device, type_, rows, k, n):
     """Integers whose sums fp32 holds exactly: every product is there once, and nothing else."""
-    for pad in (0, 3, 8) if rows < 2000 else (8,):
+    for pad in (0, 3, 8) if rows < 2000 and n < 4000 else (8,) if rows > 2000 else (0,):
         x = torch.randint(-8, 9, (rows, k), generator=gen(k + pad)).double()
         w = torch.randint(-8, 9, (n, k), generator=gen(n + pad)).double()
         b = torch.randint(-99, 99, (n,), generator=gen(7)).double()
