@@ -769,19 +769,48 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
     if constexpr (kMx) xs[e] = a.x_scales + row * a.ld_xs;
   }
   f32x4v acc[NT][MT] = {};
-  for (int kt0 = wave; kt0 < a.k_tiles; kt0 += kWaves * kBatch) {
+  // A batch is every eighth k-tile, in 8 bits neighbours: their scales are one load per row.
+  constexpr int kNext = kMx ? 1 : kWaves;
+  for (int kt0 = wave * (kMx ? kBatch : 1); kt0 < a.k_tiles; kt0 += kWaves * kBatch) {
     u32x4 qw[kBatch][NT][2], qx[kBatch][MT][2];
     uint32_t sw[kBatch][NT], sx[kBatch][MT];
+    if constexpr (kMx) {
+      typedef uint32_t words __attribute__((ext_vector_type(kBatch)));
+      typedef words words_byte __attribute__((aligned(1)));
+#pragma unroll
+      for (int f = 0; f < NT; ++f) {  // (whole fours of k-tiles are there)
+        const words q = *reinterpret_cast<const words *>(a.w_scales + ((int64_t)(kt0 >> 2) * a.n_pad + n0 + f * 16 + r16) * 4 + (kt0 & 3));
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) sw[u][f] = q[u];
+      }
+      const bool whole = (kt0 + kBatch) * 4 <= all_groups;
+#pragma unroll
+      for (int e = 0; e < MT; ++e) {
+        if (whole) {
+          const words q = *reinterpret_cast<const words_byte *>(xs[e] + kt0 * 4);
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) sx[u][e] = q[u];
+        } else {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int kt = kt0 + u;
+            sx[u][e] = 0;
+            if ((kt + 1) * 4 <= all_groups) sx[u][e] = *reinterpret_cast<const u32_byte *>(xs[e] + kt * 4);
+            else if (kt < a.k_tiles) sx[u][e] = load_scales(xs[e], kt, all_groups);
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int kt = kt0 + u * kWaves;
+      const int kt = kt0 + u * kNext;
       if (kt >= a.k_tiles) continue;
       const uint8_t *p = w + (int64_t)kt * a.n_pad * kTileBytes;
 #pragma unroll
       for (int f = 0; f < NT; ++f) {
         qw[u][f][0] = *reinterpret_cast<const u32x4 *>(p + f * 16 * kTileBytes);
         qw[u][f][1] = *reinterpret_cast<const u32x4 *>(p + f * 16 * kTileBytes + 64);
-        sw[u][f] = kMx ? a.w_scales[((int64_t)(kt >> 2) * a.n_pad + n0 + f * 16 + r16) * 4 + (kt & 3)] : 0;
+        if constexpr (!kMx) sw[u][f] = 0;
       }
       const int at = kt * kTileBytes + g * 16;
       if ((kt + 1) * kTileBytes <= bytes) {
@@ -789,22 +818,20 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
         for (int e = 0; e < MT; ++e) {
           qx[u][e][0] = *reinterpret_cast<const u32x4_byte *>(x[e] + at);
           qx[u][e][1] = *reinterpret_cast<const u32x4_byte *>(x[e] + at + 64);
-          sx[u][e] = 0;
-          if constexpr (kMx) sx[u][e] = *reinterpret_cast<const u32_byte *>(xs[e] + kt * 4);
+          if constexpr (!kMx) sx[u][e] = 0;
         }
       } else {
 #pragma unroll
         for (int e = 0; e < MT; ++e) {
           qx[u][e][0] = load_chunk(x[e], at, bytes);
           qx[u][e][1] = load_chunk(x[e], at + 64, bytes);
-          sx[u][e] = 0;
-          if constexpr (kMx) sx[u][e] = load_scales(xs[e], kt, all_groups);
+          if constexpr (!kMx) sx[u][e] = 0;
         }
       }
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      if (kt0 + u * kWaves >= a.k_tiles) break;
+      if (kt0 + u * kNext >= a.k_tiles) break;
       Operand<KIND> fw[NT];
 #pragma unroll
       for (int f = 0; f < NT; ++f) fw[f].set(qw[u][f][0], qw[u][f][1], sw[u][f], g);
@@ -893,52 +920,72 @@ int LaunchThin(const LinearArgs &args, hipStream_t st) {
   });
 }
 
-// Up to 32 rows: the thin kernel, with 32 outputs a block where that leaves a block for each
-// compute unit (16 x 8192 x 8192 bf16: 24.9 us with 32, 31.1 with 16; 16 x 4096 x 4096 mx8, 128 blocks
-// of 32: 9.0 us, 256 of 16: 7.3) or a group of 32 8-bit outputs has to stay together.  The
-// pipelined kernel of 64 x 64 takes 18.0 us for 64 x 4096 x 4096 bf16, the thin one 24.4; at 32 rows
-// of mx8 13.1 and 9.7.
-//
-// More rows: the form of the pipelined kernel with the least estimated time, from the turns that the
-// busiest compute unit has to take.  Microseconds per k-tile and per turn, measured in bf16 at the
-// sizes behind each line; only their relation matters.
+// The form with the least estimated time, from the turns that the busiest compute unit has to take.
+// Microseconds per k-tile and per turn, measured in bf16 at the sizes behind each line (less the
+// 2.2 that every launch takes); only their relation matters.
 //   256 x 256, 8 waves                      1.62 kt + 7    35554 x 2000 x 8600: 1118 (measured 1157)
 //   128 x 128, 4 waves, alone on its unit   0.65 kt + 2    1024 x 4096 x 4096: 44 (44.5)
 //              two of them                  0.95 kt + 4    4096 x 2048 x 2048: 34 (34.4)
 //   128 x 128, 2 groups of 4 waves          0.55 kt + 3    1024 x 4096 x 4096: 38 (38.7)
-//   64 x 64, 4 waves, alone                 0.31 kt + 1    300 x 360 x 2000: 5.9 (5.5, launch and all)
+//   64 x 64, 4 waves, alone                 0.31 kt + 1    300 x 360 x 2000: 2.9 (5.5 with the launch)
 //            two of them                    0.38 kt + 2    1024 x 4096 x 4096: 53 (54)
-//   64 x 64, 2 groups of 4 waves            0.24 kt + 2    256 x 4096 x 4096: 17 (18.3)
+//   64 x 64, 2 groups of 4 waves            0.27 kt + 1.5  32 x 4096 x 16384: 21 (22.4 with it)
 // Rows of x that do not start and end on 16 bytes go through registers, in two forms:
 //   64 x 64, four blocks a unit             0.36 kt each   1237 x 1999 x 2001 bf16: 30.0 (128 x 128: 39.5)
+//            alone                          0.45 kt        64 x 2000 x 1024: 14.4 (16.0 with it)
 //   128 x 128, alone / two of them   1.25 kt / 2.0 kt      2000 x 2002 x 4096 mx8: 32.0 (64 x 64: 53.1)
+// The thin kernel, whatever the rows' places; the second figure where they are not on 16 bytes
+// (sizes and times as above, all with the launch), and 0.5 a turn:
+//   16 rows x 16 outputs                    0.12, 0.18 kt  64 x 4096 x 1024: 10.3 (64 x 64: 21.3)
+//   16 rows x 32 outputs                    0.19, 0.20 kt  16 x 8192 x 8192: 25.3 (16 x 16: 31.1)
+//   32 rows x 16 outputs                    0.18, 0.33 kt  128 x 4096 x 1024: 14.0 (64 x 64: 21.4)
+//   32 rows x 32 outputs                    0.25, 0.37 kt  64 x 4096 x 4096: 18.0 (64 x 64: 21.7)
+//   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 21.0 (33.3)
+// 8-bit operands widened to 16 cost the tile kernels 2.9 times a k-tile, whose waves widen the same
+// outputs' over and over, and the thin one 1.35 times: 2.1 in relation.
 }  // namespace
 
 template <int KIND>
 int LaunchLinear(const LinearArgs &a, hipStream_t st) {
-  if (a.rows <= 32) {
-    const bool wide = a.out_type == AMLIKE_MX8 || a.n_pad / 32 >= NumComputeUnits();
-    if (a.rows <= 16) return wide ? LaunchThin<KIND, 2, 1>(a, st) : LaunchThin<KIND, 1, 1>(a, st);
-    return wide ? LaunchThin<KIND, 2, 2>(a, st) : LaunchThin<KIND, 1, 2>(a, st);
-  }
-  if (a.ldx > 1 << 22 || a.ld_xs > 1 << 22) return LaunchThin<KIND, 2, 4>(a, st);  // a tile's rows have to lie within 32 bits
-  const double units = std::max(1, NumComputeUnits()), kt = a.k_tiles;
-  auto turns = [&](int edge) {
-    return std::ceil((double)(((int64_t)a.rows + edge - 1) / edge * ((a.n_pad + edge - 1) / edge)) / units);
+  const double units = std::max(1, NumComputeUnits()), k_tiles = a.k_tiles, kt = KIND == kMx8Exact ? 2.1 * k_tiles : k_tiles;
+  auto turns = [&](int rows, int outputs) {
+    return std::ceil((double)(((int64_t)a.rows + rows - 1) / rows * ((a.n_pad + outputs - 1) / outputs)) / units);
   };
-  const double t256 = turns(256), t128 = turns(128), t64 = turns(64);
-  const double cost[5] = {t256 * (1.62 * kt + 7), t128 <= 1 ? 0.65 * kt + 2 : std::ceil(t128 / 2) * (0.95 * kt + 4), t128 * (0.55 * kt + 3),
-                          t64 <= 1 ? 0.31 * kt + 1 : std::ceil(t64 / 2) * (0.38 * kt + 2), t64 * (0.24 * kt + 2)};
-  if (!Copyable(a, KIND))
-    return std::ceil(t64 / 4) * std::min(t64, 4.0) * 0.36 < (t128 <= 1 ? 1.25 : std::ceil(t128 / 2) * 2.0)
-               ? LaunchPipe<KIND, 1, 4, 1, 2, 1, false>(a, st)
-               : LaunchPipe<KIND, 2, 2, 4, 2, 1, false>(a, st);
+  const bool copy = Copyable(a, KIND);
+  auto thin_cost = [&](int rows, int outputs, double on_16, double off) {
+    return turns(rows, outputs) * ((copy ? on_16 : off) * k_tiles + 0.5);
+  };
+  const double thin[5] = {thin_cost(16, 16, 0.12, 0.18), thin_cost(16, 32, 0.19, 0.20), thin_cost(32, 16, 0.18, 0.33),
+                          thin_cost(32, 32, 0.25, 0.37), thin_cost(64, 32, 0.35, 0.66)};
+  const double t256 = turns(256, 256), t128 = turns(128, 128), t64 = turns(64, 64);
+  double tile[7] = {t256 * (1.62 * kt + 7),
+                    t128 <= 1 ? 0.65 * kt + 2 : std::ceil(t128 / 2) * (0.95 * kt + 4),
+                    t128 * (0.55 * kt + 3),
+                    t64 <= 1 ? 0.31 * kt + 1 : std::ceil(t64 / 2) * (0.38 * kt + 2),
+                    t64 * (0.27 * kt + 1.5),
+                    t64 <= 1 ? 0.45 * kt : std::ceil(t64 / 4) * std::min(t64, 4.0) * 0.36 * kt,
+                    t128 <= 1 ? 1.25 * kt : std::ceil(t128 / 2) * 2.0 * kt};
   // (with widened 8-bit operands the largest tile's registers do not suffice)
-  const int first = KIND == kMx8Exact ? 1 : 0, best = (int)(std::min_element(cost + first, cost + 5) - cost);
+  const int first = !copy ? 5 : KIND == kMx8Exact ? 1 : 0, last = copy ? 5 : 7;
+  const int best = (int)(std::min_element(tile + first, tile + last) - tile);
+  // (a group of 32 8-bit outputs stays in one block)
+  int few = a.out_type == AMLIKE_MX8 ? 1 : 0;
+  for (int i = few + 1; i < 5; ++i)
+    if (thin[i] < thin[few] && (i != 2 || a.out_type != AMLIKE_MX8)) few = i;
+  // (the tile kernel addresses a tile's rows with 32 bits)
+  if (thin[few] < tile[best] || a.ldx > 1 << 22 || a.ld_xs > 1 << 22) {
+    if (few == 0) return LaunchThin<KIND, 1, 1>(a, st);
+    if (few == 1) return LaunchThin<KIND, 2, 1>(a, st);
+    if (few == 2) return LaunchThin<KIND, 1, 2>(a, st);
+    if (few == 3) return LaunchThin<KIND, 2, 2>(a, st);
+    return LaunchThin<KIND, 2, 4>(a, st);
+  }
   if (best == 1) return LaunchPipe<KIND, 2, 2, 4, 2, 1>(a, st);
   if (best == 2) return LaunchPipe<KIND, 2, 2, 4, 2, 2>(a, st);
   if (best == 3) return LaunchPipe<KIND, 1, 4, 1, 4, 1>(a, st);
   if (best == 4) return LaunchPipe<KIND, 1, 4, 1, 4, 2>(a, st);
+  if (best == 5) return LaunchPipe<KIND, 1, 4, 1, 2, 1, false>(a, st);
+  if (best == 6) return LaunchPipe<KIND, 2, 2, 4, 2, 1, false>(a, st);
   if constexpr (KIND != kMx8Exact) return LaunchPipe<KIND, 4, 2, 8, 2, 1>(a, st);
   return AMLIKE_EINVAL;
 }

@@ -252,6 +252,31 @@ def test_linear_is_exact_on_small_integers(amlike_device, type_, rows, k, n):
                 assert torch.equal(out.values(), torch.relu((x @ w.t()) * p * q).bfloat16().double()), (pad,)
 
 
+# Sizes that are large enough for every form of the tile kernel on 256 compute units (in 8 bits with twice
+# the columns): k-tiles of one block and of two groups of waves, 64, 128 and 256 wide, one tile a
+# block and several; the last is for rows that start anywhere.
+FORMS = [(990, 200, 2000, 16), (60000, 200, 60, 16), (500, 1000, 2000, 16), (3990, 200, 1990, 16), (4090, 200, 4600, 16), (1990, 1000, 1990, 16),
+         (90000, 504, 120, 16), (4090, 1000, 4090, 16), (8000, 200, 8000, 16), (500, 1017, 2000, 3)]
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16", "mx8"])
+@pytest.mark.parametrize("rows,k,n,pad", FORMS)
+def test_linear_forms_are_exact_on_small_integers(amlike_device, type_, rows, k, n, pad):
+    k *= 2 if type_ == "mx8" else 1
+    x = torch.randint(-8, 9, (rows, k), generator=gen(61)).double()
+    w = torch.randint(-8, 9, (n, k), generator=gen(62)).double()
+    b = torch.randint(-99, 99, (n,), generator=gen(63)).double()
+    lin = dense.Linear(w.numpy(), b.numpy(), type_)
+    dx = U.DeviceMatrix(rows, k, type_, pad, fill=x)
+    want = x @ w.t() + b
+    for tout in ("f32", "bf16", "mx8") if rows < 5000 else ("f32", "bf16"):
+        out = U.DeviceMatrix(rows, n, tout, pad)
+        lin.ApplyDevice(dx.m, rows, out.m)
+        torch.cuda.synchronize()
+        U.check_output(out, want, torch.zeros_like(want)) if tout == "mx8" else U.assert_close(out.values(), U.rounded(want, tout), 0.0, tout)
+        out.assert_rest_untouched()
+
+
 @pytest.mark.parametrize("type_", ["bf16", "f16", "mx8"])
 @pytest.mark.parametrize("tout,act,tres", [("f32", "none", None), ("f32", "gelu", "f32"), ("f32", "tanh", "bf16"), ("f32", "silu", None),
                                            ("f32", "sigmoid", "f16"), ("bf16", "gelu", "bf16"), ("bf16", "relu", None), ("f16", "silu", "f16"),
