@@ -750,15 +750,20 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
 // (few rows: HBM) and of x (more rows: every block reads all of its rows from L2), so there is
 // nothing for LDS to save; eight waves with kBatch k-tiles in flight each cover the latency.
 template <int KIND, int NT, int MT>
-__global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_tiles) {
+__global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_tiles, int n_tiles) {
   constexpr int kWaves = 8, kCols = 16 * NT, kRows = 16 * MT, kBatch = MT >= 4 ? 2 : 4;
   constexpr bool kMx = IsMx8(KIND);
   typedef u32x4 u32x4_byte __attribute__((aligned(1)));
   typedef uint32_t u32_byte __attribute__((aligned(1)));
   __shared__ float s_c[kWaves][kRows][kCols + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
-  const int n0 = (int)(blockIdx.x / m_tiles) * kCols;
-  const int64_t m0 = (int64_t)(blockIdx.x % m_tiles) * kRows;
+  // Strips of the larger operand are dealt to the XCDs (blocks b, b + 8 ..), each with all its tiles.
+  const bool by_rows = m_tiles > n_tiles;
+  const int inner = by_rows ? n_tiles : m_tiles, j = blockIdx.x >> 3;
+  const int strip = j / inner * 8 + (blockIdx.x & 7), in = j % inner;
+  if (strip >= (by_rows ? m_tiles : n_tiles)) return;
+  const int n0 = (by_rows ? in : strip) * kCols;
+  const int64_t m0 = (int64_t)(by_rows ? strip : in) * kRows;
   const int bytes = a.k * (kMx ? 1 : 2), all_groups = (a.k + 31) >> 5;
   const uint8_t *w = a.w + (int64_t)(n0 + r16) * kTileBytes + g * 16;
   const uint8_t *x[MT], *xs[kMx ? MT : 1];
@@ -870,11 +875,11 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
 
 namespace {
 
-// Calls `launch` on stretches of the rows, all of them but for outputs beyond 2^33 elements: a grid
-// holds less than 2^32 threads, 2^23 blocks of 512.
+// Calls `launch` on stretches of the rows, all of them but for outputs beyond 2^22 blocks of `tile`
+// elements: a grid holds less than 2^32 threads, 2^23 blocks of 512.
 template <typename F>
-int ByRows(LinearArgs a, F launch) {
-  const int64_t most = std::max<int64_t>(((int64_t)1 << 33) / a.n_pad / 256 * 256, 256);
+int ByRows(LinearArgs a, int tile, F launch) {
+  const int64_t most = std::max<int64_t>(((int64_t)1 << 22) * tile / a.n_pad / 256 * 256, 256);
   const int64_t rows = a.rows;
   const int rb = a.res_type < 0 ? 0 : TypeBytes(a.res_type), ob = TypeBytes(a.out_type);
   for (int64_t r = 0; r < rows; r += most) {
@@ -891,7 +896,7 @@ int ByRows(LinearArgs a, F launch) {
 
 template <int KIND, int WN, int WM, int MF, int STAGES, int KS, bool COPY = true>
 int LaunchPipe(const LinearArgs &args, hipStream_t st) {
-  return ByRows(args, [&](const LinearArgs &a) -> int {
+  return ByRows(args, 2048, [&](const LinearArgs &a) -> int {
     const int m_tiles = (a.rows + 16 * MF * WM - 1) / (16 * MF * WM), n_tiles = (a.n_pad + 64 * WN - 1) / (64 * WN);
     // as many blocks as the device holds at once, by waves and LDS, in eights
     constexpr int kLds = KS * (64 * WN + 16 * MF * WM) * (STAGES * kTileBytes + (IsMx8(KIND) ? 32 : 0)) + 64;
@@ -912,9 +917,10 @@ bool Copyable(const LinearArgs &a, int kind) {
 
 template <int KIND, int NT, int MT>
 int LaunchThin(const LinearArgs &args, hipStream_t st) {
-  return ByRows(args, [&](const LinearArgs &a) -> int {
-    const int m_tiles = (a.rows + 16 * MT - 1) / (16 * MT);
-    hipLaunchKernelGGL((linear_thin_kernel<KIND, NT, MT>), dim3((unsigned)m_tiles * (a.n_pad / (16 * NT))), dim3(512), 0, st, a, m_tiles);
+  return ByRows(args, 256 * NT * MT, [&](const LinearArgs &a) -> int {
+    const int m_tiles = (a.rows + 16 * MT - 1) / (16 * MT), n_tiles = a.n_pad / (16 * NT);
+    const unsigned blocks = (unsigned)((std::max(m_tiles, n_tiles) + 7) & ~7) * std::min(m_tiles, n_tiles);
+    hipLaunchKernelGGL((linear_thin_kernel<KIND, NT, MT>), dim3(blocks), dim3(512), 0, st, a, m_tiles, n_tiles);
     AMLIKE_HIP(hipGetLastError());
     return AMLIKE_OK;
   });
