@@ -746,9 +746,12 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
 
 // ---- few rows ------------------------------------------------------------------------------------------
 // 16 NT outputs x 16 MT rows per block; its eight waves share the k-tiles among them, each from
-// memory straight into registers, and add up in LDS in wave order.  What bounds it is the way of W
-// (few rows: HBM) and of x (more rows: every block reads all of its rows from L2), so there is
-// nothing for LDS to save; eight waves with kBatch k-tiles in flight each cover the latency.
+// memory straight into registers, and add up in LDS in wave order; kBatch k-tiles of each are in
+// flight.  For few rows the way of W from HBM bounds it (16 x 8192 x 8192 bf16: 24.9 us, 5.4 TB/s), for
+// small products a launch and two trips to memory (1 x 2048 x 2048 bf16: 4.6 us, of which 2.2 are any
+// launch's).  (Tried: biases and residual asked for before the k-tiles, 0; the k-tile that rows end in
+// moved out of the batches, 0; eight whole lines a load instead of sixteen halves, with lanes trading
+// pieces, -5 %.)
 template <int KIND, int NT, int MT>
 __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_tiles, int n_tiles) {
   constexpr int kWaves = 8, kCols = 16 * NT, kRows = 16 * MT, kBatch = MT >= 4 ? 2 : 4;
