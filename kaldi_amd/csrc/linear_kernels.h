@@ -89,17 +89,18 @@ struct Frag<AMLIKE_F16> {
 };
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// A 16-byte piece of e4m3 values times their scale (an e8m0 byte), as two fragments of bf16.
+// A 16-byte piece of e4m3 values times their scale (an e8m0 byte), as two fragments of bf16.  The
+// conversion takes the exponent of its scale as it stands, 2^-127 and the NaN of byte 255 included.
 __device__ __forceinline__ void widen(const u32x4 p, uint32_t scale_byte, Frag<AMLIKE_BF16>::vec out[2]) {
-  // (2^-127 is a denormal: the byte's bits in an exponent field would be 0)
-  const float s = as_float(scale_byte ? scale_byte << 23 : 0x400000u);
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const float s = as_float(scale_byte << 23);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const f32x2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)p[q], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)p[q], true);
-    out[q >> 1][(q & 1) * 4 + 0] = (__bf16)(a[0] * s);
-    out[q >> 1][(q & 1) * 4 + 1] = (__bf16)(a[1] * s);
-    out[q >> 1][(q & 1) * 4 + 2] = (__bf16)(b[0] * s);
-    out[q >> 1][(q & 1) * 4 + 3] = (__bf16)(b[1] * s);
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)p[q], s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)p[q], s, true);
+    out[q >> 1][(q & 1) * 4 + 0] = a[0];
+    out[q >> 1][(q & 1) * 4 + 1] = a[1];
+    out[q >> 1][(q & 1) * 4 + 2] = b[0];
+    out[q >> 1][(q & 1) * 4 + 3] = b[1];
   }
 }
 
@@ -949,14 +950,14 @@ int LaunchThin(const LinearArgs &args, hipStream_t st) {
 //   16 rows x 32 outputs                    0.19, 0.20 kt  16 x 8192 x 8192: 25.3 (16 x 16: 31.1)
 //   32 rows x 16 outputs                    0.18, 0.33 kt  128 x 4096 x 1024: 14.0 (64 x 64: 21.4)
 //   32 rows x 32 outputs                    0.25, 0.37 kt  64 x 4096 x 4096: 18.0 (64 x 64: 21.7)
-//   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 21.0 (33.3)
-// 8-bit operands widened to 16 cost the tile kernels 2.9 times a k-tile, whose waves widen the same
-// outputs' over and over, and the thin one 1.35 times: 2.1 in relation.
+//   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 17.0 (20.0)
+// 8-bit operands widened to 16 cost the tile kernels 1.9 times a k-tile (twice the products, and every wave
+// widens what it reads) and the thin one 1.08 times: 1.75 in relation.
 }  // namespace
 
 template <int KIND>
 int LaunchLinear(const LinearArgs &a, hipStream_t st) {
-  const double units = std::max(1, NumComputeUnits()), k_tiles = a.k_tiles, kt = KIND == kMx8Exact ? 2.1 * k_tiles : k_tiles;
+  const double units = std::max(1, NumComputeUnits()), k_tiles = a.k_tiles, kt = KIND == kMx8Exact ? 1.75 * k_tiles : k_tiles;
   auto turns = [&](int rows, int outputs) {
     return std::ceil((double)(((int64_t)a.rows + rows - 1) / rows * ((a.n_pad + outputs - 1) / outputs)) / units);
   };

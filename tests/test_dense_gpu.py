@@ -365,6 +365,26 @@ def test_linear_extreme_scales(amlike_device):
         assert torch.equal(out.values(), U.rounded(x @ wide.t(), tout))
 
 
+@pytest.mark.parametrize("rows,k,n", [(3, 96, 40), (20, 256, 64), (990, 400, 2000)])
+def test_linear_scale_bytes_at_both_ends(amlike_device, rows, k, n):
+    """Byte 0 stands for 2^-127, byte 255 for NaN: of its row alone."""
+    x, w = torch.randint(-8, 9, (rows, k), generator=gen(71)).double(), torch.randint(-8, 9, (n, k), generator=gen(72)).double()
+    w[:, ::3] = 8
+    lin = dense.Linear(w.numpy(), None, "mx8")
+    dx = U.DeviceMatrix(rows, k, "mx8", 16, fill=x)
+    dx.scales[0, :(k + 31) // 32] = 0
+    dx.scales[rows - 1, 1] = 255
+    want = dx.values()[:rows - 1] @ w.t()
+    for tout in ("f32", "bf16"):
+        out = U.DeviceMatrix(rows, n, tout)
+        lin.ApplyDevice(dx.m, rows, out.m)
+        torch.cuda.synchronize()
+        got = out.values()
+        assert torch.isnan(got[rows - 1]).all()
+        # (integers of at most 8 are held as multiples of 2^5 and more: no sum lies below 2^-122)
+        assert torch.equal(got[:rows - 1], U.rounded(want, tout))
+
+
 def test_linear_residual_in_place(amlike_device):
     x, r = U.rounded(randn(50, 96, 31), "bf16"), U.rounded(randn(50, 130, 32), "bf16")
     lin = dense.Linear((randn(130, 96, 33) / 10).numpy(), None, "bf16")
