@@ -946,10 +946,10 @@ int LaunchThin(const LinearArgs &args, hipStream_t st) {
 //   128 x 128, alone / two of them   1.25 kt / 2.0 kt      2000 x 2002 x 4096 mx8: 32.0 (64 x 64: 53.1)
 // The thin kernel, whatever the rows' places; the second figure where they are not on 16 bytes
 // (sizes and times as above, all with the launch), and 0.5 a turn:
-//   16 rows x 16 outputs                    0.12, 0.18 kt  64 x 4096 x 1024: 10.3 (64 x 64: 21.3)
-//   16 rows x 32 outputs                    0.19, 0.20 kt  16 x 8192 x 8192: 25.3 (16 x 16: 31.1)
-//   32 rows x 16 outputs                    0.18, 0.33 kt  128 x 4096 x 1024: 14.0 (64 x 64: 21.4)
-//   32 rows x 32 outputs                    0.25, 0.37 kt  64 x 4096 x 4096: 18.0 (64 x 64: 21.7)
+//   16 rows x 16 outputs                    0.12, 0.18 kt  64 x 4096 x 1024: 9.5 (64 x 64: 21.3)
+//   16 rows x 32 outputs                    0.19, 0.20 kt  16 x 8192 x 8192: 24.9 (16 x 16: 31.1)
+//   32 rows x 16 outputs                    0.18, 0.33 kt  128 x 4096 x 1024: 13.0 (64 x 64: 21.4)
+//   32 rows x 32 outputs                    0.25, 0.37 kt  64 x 4096 x 4096: 17.5 (64 x 64: 21.7)
 //   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 17.0 (20.0)
 // 8-bit operands widened to 16 cost the tile kernels 1.9 times a k-tile (twice the products, and every wave
 // widens what it reads) and the thin one 1.08 times: 1.75 in relation.
