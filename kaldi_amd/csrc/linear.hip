@@ -42,13 +42,27 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const uint8_t *__restr
     if (no) ctl_or(bad, 1);
   }
 }
-__global__ __launch_bounds__(256) void linear_pack_scales_kernel(const uint8_t *__restrict__ src, int n, int k, int n_pad,
-                                                                 int64_t words, uint32_t *__restrict__ dst) {
+// One word (four groups' scales) per thread.  A group of zeros has 2^0 here instead of the format's smallest
+// scale: the same products, and nothing for a kernel to look at closely.
+__global__ __launch_bounds__(256) void linear_pack_scales_kernel(const uint8_t *__restrict__ src, const uint8_t *__restrict__ values,
+                                                                 int n, int k, int n_pad, int64_t words, uint32_t *__restrict__ dst) {
   const int groups = (k + 31) >> 5;
   for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < words; p += (int64_t)gridDim.x * 256) {
     const int64_t line = p >> 2;
     const int four = (int)(line / n_pad), row = (int)(line - (int64_t)four * n_pad);
-    dst[p] = row < n ? load_scales(src + (int64_t)row * groups, four * 4 + (int)(p & 3), groups) : 0x7f7f7f7fu;
+    uint32_t s = 0x7f7f7f7fu;
+    if (row < n) {
+      const int kt = four * 4 + (int)(p & 3);
+      s = load_scales(src + (int64_t)row * groups, kt, groups);
+      for (int i = 0; i < 4; ++i) {
+        if ((s >> (8 * i) & 0xff) != 0) continue;
+        const int first = (kt * 4 + i) * 32;
+        uint8_t any = 0;
+        for (int c = first; c < min(first + 32, k); ++c) any |= values[(int64_t)row * k + c] & 0x7f;
+        if (any == 0) s |= 0x7fu << (8 * i);
+      }
+    }
+    dst[p] = s;
   }
 }
 
@@ -100,7 +114,8 @@ int PackWeights(amlike_linear *h, const float *weights, int64_t ld, const float 
       const int64_t words = (int64_t)((h->k_tiles + 3) & ~3) * h->n_pad;
       AMLIKE_HIP(hipMalloc(reinterpret_cast<void **>(&h->d_scales), (size_t)words * 4));
       hipLaunchKernelGGL(linear_pack_scales_kernel, dim3((unsigned)std::min<int64_t>((words + 255) / 256, 1 << 16)), dim3(256), 0,
-                         h->stream, static_cast<const uint8_t *>(scales.ptr), h->n, h->k, h->n_pad, words, h->d_scales);
+                         h->stream, static_cast<const uint8_t *>(scales.ptr), static_cast<const uint8_t *>(typed.ptr), h->n, h->k,
+                         h->n_pad, words, h->d_scales);
       AMLIKE_HIP(hipGetLastError());
     }
     int bad = 0;

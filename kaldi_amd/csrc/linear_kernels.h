@@ -14,9 +14,12 @@
 // is whole), which leaves a relative error of about 1.5e-5 in a sum of normal values whatever its
 // length: far below the rounding of a 16-bit (2^-9, 2^-12 on average) or 8-bit output, too much for
 // an fp32 one.  For an fp32 output the 8-bit operands are therefore widened to bf16, which holds
-// value times scale exactly, and multiplied there (kMx8Exact), at half the matrix rate.
+// value times scale exactly but for scales at the ends of their range (is_far_x), and multiplied there
+// (kMx8Exact), at half the matrix rate.  A wave that met such a scale takes its sums once more, group
+// by group (far_sums).
 //   W:      [k-tile][row, padded to 64][128 bytes], zeros behind both ends
-//   scales: [k-tile / 4][row, padded to 64][k-tile % 4][4 bytes], 2^0 behind both ends  (8 bits only)
+//   scales: [k-tile / 4][row, padded to 64][k-tile % 4][4 bytes], 2^0 behind both ends and for groups
+//           of zeros  (8 bits only)
 //
 // This header holds the kernels and the choice between them; each kind of product is compiled in a file
 // of its own (linear_bf16.hip ...), the host side is linear.hip.
@@ -89,11 +92,11 @@ struct Frag<AMLIKE_F16> {
 };
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// A 16-byte piece of e4m3 values times their scale (an e8m0 byte), as two fragments of bf16.  The
-// conversion takes the exponent of its scale as it stands, 2^-127 and the NaN of byte 255 included.
-__device__ __forceinline__ void widen(const u32x4 p, uint32_t scale_byte, Frag<AMLIKE_BF16>::vec out[2]) {
+// A 16-byte piece of e4m3 values times 2^(scale byte - 127 + lift), as two fragments of bf16.  The
+// conversion takes the exponent of its scale as it stands.
+__device__ __forceinline__ void widen(const u32x4 p, uint32_t scale_byte, int lift, Frag<AMLIKE_BF16>::vec out[2]) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const float s = as_float(scale_byte << 23);
+  const float s = as_float((scale_byte << 23) + ((uint32_t)lift << 23));
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)p[q], s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)p[q], s, true);
@@ -104,13 +107,26 @@ __device__ __forceinline__ void widen(const u32x4 p, uint32_t scale_byte, Frag<A
   }
 }
 
+// bf16 holds multiples of 2^-133 below 2^128, an 8-bit value is a multiple of 2^-9 up to 448 times
+// 2^(byte - 127).  With x lifted by 2^3, and W lowered by as much, every value of x under the bytes 0
+// (rows and groups of zeros have it) to 243 fits, and every one of W under the bytes 6 to 249.  Beyond,
+// x would become infinite and W lose its last bits.
+constexpr int kLift = 3;
+// Whether one of four scale bytes of x is 244 or more (NaN's 255 too): its low seven bits plus 12
+// reach the eighth, and that is set.
+__device__ __forceinline__ bool is_far_x(uint32_t scales) {
+  return (((scales & 0x7f7f7f7fu) + 0x0c0c0c0cu) & scales & 0x80808080u) != 0;
+}
+// Whether one of four scale bytes of W is below 6.  (Packed W has no byte over 247.)
+__device__ __forceinline__ bool is_far_w(uint32_t scales) { return ((scales - 0x06060606u) & ~scales & 0x80808080u) != 0; }
+
 // What a lane feeds the matrix instructions from pieces g and g + 4 of a row in one k-tile, and the
-// word of the row's four scales.
+// word of the row's four scales.  lift: kLift for x, -kLift for W.
 template <int KIND>
 struct Operand {
   u32x4 p[2];
   int scale;
-  __device__ __forceinline__ void set(u32x4 p0, u32x4 p1, uint32_t scales, int g) {
+  __device__ __forceinline__ void set(u32x4 p0, u32x4 p1, uint32_t scales, int g, int /*lift*/) {
     p[0] = p0;
     p[1] = p1;
     scale = (int)(scales >> (8 * g));  // the instruction takes the lowest byte
@@ -119,9 +135,9 @@ struct Operand {
 template <>
 struct Operand<kMx8Exact> {
   Frag<AMLIKE_BF16>::vec v[4];
-  __device__ __forceinline__ void set(u32x4 p0, u32x4 p1, uint32_t scales, int g) {
-    widen(p0, scales >> (8 * (g >> 1)) & 0xff, v);  // piece c holds columns of group c / 2
-    widen(p1, scales >> (16 + 8 * (g >> 1)) & 0xff, v + 2);
+  __device__ __forceinline__ void set(u32x4 p0, u32x4 p1, uint32_t scales, int g, int lift) {
+    widen(p0, scales >> (8 * (g >> 1)) & 0xff, lift, v);  // piece c holds columns of group c / 2
+    widen(p1, scales >> (16 + 8 * (g >> 1)) & 0xff, lift, v + 2);
   }
 };
 
@@ -146,6 +162,75 @@ __device__ __forceinline__ f32x4v tile_product(const Operand<TYPE> &ow, const Op
       else c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
     return c;
+  }
+}
+
+// ---- 8 bits as bf16: scales at the ends of their range ------------------------------------------------
+// tile_product of widened 8-bit operands for any scales: per group of 32 columns the sum of the unscaled
+// values' products, which then moves by both scales at once.  Rows of x that need it not keep the
+// ordinary product's bits, so that no row depends on its neighbours; where a row of W needs it, all do.
+__device__ __forceinline__ f32x4v far_product(const u32x4 w[2], uint32_t sw, const u32x4 x[2], uint32_t sx, int g, f32x4v c) {
+  const bool far = __ballot(is_far_w(sw)) != 0 || is_far_x(sx);  // (results of row r16 of x are in the lanes that hold its scales)
+  f32x4v ordinary;
+  {
+    Operand<kMx8Exact> ow, ox;
+    ow.set(w[0], w[1], sw, g, -kLift);
+    ox.set(x[0], x[1], sx, g, kLift);
+    ordinary = tile_product<kMx8Exact>(ow, ox, c);
+  }
+  f32x4v sum = c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    __builtin_amdgcn_sched_barrier(0);  // (few registers rather than speed)
+    f32x4v part = {0, 0, 0, 0};
+    Frag<AMLIKE_BF16>::vec vw[2], vx[2];
+    widen(w[j >> 1], 127, 0, vw);
+    widen(x[j >> 1], 127, 0, vx);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if ((g >> 1) != (j & 1)) vx[h] = Frag<AMLIKE_BF16>::vec{};  // the other lanes hold group j
+      part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vw[h], vx[h], part, 0, 0, 0);
+    }
+    const int bx = (int)(sx >> (8 * j) & 0xff);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int bw = (int)((uint32_t)__shfl((int)sw, 4 * g + i) >> (8 * j) & 0xff);
+      sum[i] += bx == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(part[i], bx + bw - 254);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = far ? sum[i] : ordinary[i];
+  return sum;
+}
+
+// A wave's sums once more for any scales, over the k-tiles of `each_tile` in the same order as before:
+// fragment f of W holds outputs n + 16 f .., fragment e of x rows m + 16 e .. up to `last`.  The
+// accumulators go round, because registers have to be named and the body is to be there once.
+// Apart from the main loops on purpose: in them, it cost 20 registers and more.
+template <int F, int E, typename Start, typename Tiles>
+__device__ __forceinline__ void far_sums(const LinearArgs &a, int64_t m, int64_t last, int n, int r16, int g, f32x4v (&acc)[F][E],
+                                         Start start, Tiles each_tile) {
+  const int groups = (a.k + 31) >> 5;
+#if __HIP_DEVICE_COMPILE__
+  asm volatile("" : "+v"(r16), "+v"(g));  // (or the addresses below are made, and kept, before the main loop)
+#endif
+#pragma clang loop unroll(disable)
+  for (int i = 0; i < F * E; ++i) {
+    const int out = min(n + i / E * 16 + r16, a.n_pad - 1);  // (behind the padded end: of no output)
+    const int64_t row = min(m + i % E * 16 + r16, last);
+    const uint8_t *x = a.x + row * a.ldx, *xs = a.x_scales + row * a.ld_xs;
+    f32x4v c = start(i / E, g);
+    each_tile([&](int kt) __attribute__((always_inline)) {
+      const uint8_t *pw = a.w + ((int64_t)kt * a.n_pad + out) * kTileBytes + g * 16;
+      const u32x4 qw[2] = {*reinterpret_cast<const u32x4 *>(pw), *reinterpret_cast<const u32x4 *>(pw + 64)};
+      const uint32_t sw = a.w_scales[((int64_t)(kt >> 2) * a.n_pad + out) * 4 + (kt & 3)];
+      const int at = kt * kTileBytes + g * 16;
+      const u32x4 qx[2] = {load_chunk(x, at, a.k), load_chunk(x, at + 64, a.k)};
+      c = far_product(qw, sw, qx, load_scales(xs, kt, groups), g, c);
+    });
+#pragma unroll
+    for (int j = 0; j < F * E - 1; ++j) acc[j / E][j % E] = acc[(j + 1) / E][(j + 1) % E];
+    acc[F - 1][E - 1] = c;
   }
 }
 
@@ -659,7 +744,7 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
 #pragma unroll
       for (int e = 0; e < MF; ++e) acc[f][e] = ks == 0 ? bias[f] : f32x4v{0, 0, 0, 0};
     }
-    auto operand = [&](int step, const u32x4 *tile, int row, int turn, int scale_row) __attribute__((always_inline)) {
+    auto operand = [&](int step, const u32x4 *tile, int row, int turn, int scale_row, int lift) __attribute__((always_inline)) {
       Operand<KIND> o;
       uint32_t sc = 0;
       if constexpr (kMx) {
@@ -669,9 +754,10 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
           if (groups < 4) sc = (sc & ~(~0u << (8 * groups))) | (0x7f7f7f7fu << (8 * groups));
         }
       }
-      o.set(tile[row * kChunks + (g ^ turn)], tile[row * kChunks + (g ^ 4 ^ turn)], sc, g);
+      o.set(tile[row * kChunks + (g ^ turn)], tile[row * kChunks + (g ^ 4 ^ turn)], sc, g, lift);
       return o;
     };
+    bool far = false;  // kMx8Exact: whether far_sums is needed (this lane's part of it)
     int step = 0;
 #if __HIP_DEVICE_COMPILE__
     asm volatile("" : "+s"(step));  // (one copy of the loop's body: the first steps are not to be peeled off)
@@ -694,18 +780,42 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>))
       const u32x4 *tw = s_tiles[ks][b], *tx = tw + BN * kChunks;
       Operand<KIND> fw[4];
 #pragma unroll
-      for (int f = 0; f < 4; ++f) fw[f] = operand(step, tw, row_w[f], turn_w(row_w[f]), scale_place(row_w[f]));
+      for (int f = 0; f < 4; ++f) fw[f] = operand(step, tw, row_w[f], turn_w(row_w[f]), scale_place(row_w[f]), -kLift);
 #pragma unroll
       for (int e = 0; e < MF; ++e) {
-        const Operand<KIND> fx = operand(step, tx, wm * 16 * MF + e * 16 + r16, turn_x(r16), BN + wm * 16 * MF + e * 16 + r16);
+        const Operand<KIND> fx = operand(step, tx, wm * 16 * MF + e * 16 + r16, turn_x(r16), BN + wm * 16 * MF + e * 16 + r16, kLift);
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[f][e] = tile_product<KIND>(fw[f], fx, acc[f][e]);
+      }
+      if constexpr (KIND == kMx8Exact) {
+        if ((step & 3) == 0) {  // the scales of this k-tile and the next three: lane (r, q) looks at k-tile step + q of its rows
+          int r = r16, q = g;
+#if __HIP_DEVICE_COMPILE__
+          asm volatile("" : "+v"(r), "+v"(q));  // (or the addresses below stay in registers through the k-tiles)
+#endif
+          const u32x4 *scales = s_scales[ks][step >> 2 & 1];
+          const int there = ((a.k + 31) >> 5) - (ks * steps + step + q) * 4;  // groups that rows of x have from there on
+          const uint32_t mask = there >= 4 ? ~0u : there <= 0 ? 0u : ~(~0u << (8 * there));
+#pragma unroll
+          for (int f = 0; f < 4; ++f) far |= is_far_w(scales[scale_place(wn * 64 + fragment_output(4, f, r))][q]);
+#pragma unroll
+          for (int e = 0; e < MF; ++e) far |= is_far_x(scales[BN + (wm * MF + e) * 16 + r][q] & mask);
+        }
       }
       }
       if (ahead) put(step + STAGES - 1, held);  // (where nobody reads now: the barriers of this turn and the next)
     }
     const int64_t m = m0 + wm * 16 * MF;
     const int n = n0 + wn * 64;
+    if constexpr (KIND == kMx8Exact) {
+      if (__builtin_expect(__ballot(far) != 0, 0))
+        far_sums(a, m, m0 + last_row(), n, r16, g, acc, [&](int f, int q) {
+          return ks == 0 ? *reinterpret_cast<const f32x4v *>(a.bias + min(n + f * 16 + q * 4, a.n_pad - 4)) : f32x4v{0, 0, 0, 0};
+        }, [&](auto tile) __attribute__((always_inline)) {
+#pragma clang loop unroll(disable)
+          for (int kt = ks * steps; kt < min((ks + 1) * steps, a.k_tiles); ++kt) tile(kt);
+        });
+    }
     if constexpr (KS > 1) {  // the first group adds the others' sums to its own, in their order
       f32x4v *part = reinterpret_cast<f32x4v *>(s_tiles);
       wait_lds();
@@ -778,6 +888,7 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
     if constexpr (kMx) xs[e] = a.x_scales + row * a.ld_xs;
   }
   f32x4v acc[NT][MT] = {};
+  bool far = false;  // kMx8Exact: whether far_sums is needed (this lane's part of it)
   // A batch is every eighth k-tile, in 8 bits neighbours: their scales are one load per row.
   constexpr int kNext = kMx ? 1 : kWaves;
   for (int kt0 = wave * (kMx ? kBatch : 1); kt0 < a.k_tiles; kt0 += kWaves * kBatch) {
@@ -838,20 +949,39 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
         }
       }
     }
+    if constexpr (KIND == kMx8Exact) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {  // (behind the last k-tile: W's are 2^0, those of x 0)
+#pragma unroll
+        for (int f = 0; f < NT; ++f) far |= is_far_w(sw[u][f]);
+#pragma unroll
+        for (int e = 0; e < MT; ++e) far |= is_far_x(sx[u][e]);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       if (kt0 + u * kNext >= a.k_tiles) break;
       Operand<KIND> fw[NT];
 #pragma unroll
-      for (int f = 0; f < NT; ++f) fw[f].set(qw[u][f][0], qw[u][f][1], sw[u][f], g);
+      for (int f = 0; f < NT; ++f) fw[f].set(qw[u][f][0], qw[u][f][1], sw[u][f], g, -kLift);
 #pragma unroll
       for (int e = 0; e < MT; ++e) {
         Operand<KIND> fx;
-        fx.set(qx[u][e][0], qx[u][e][1], sx[u][e], g);
+        fx.set(qx[u][e][0], qx[u][e][1], sx[u][e], g, kLift);
 #pragma unroll
         for (int f = 0; f < NT; ++f) acc[f][e] = tile_product<KIND>(fw[f], fx, acc[f][e]);
       }
     }
+  }
+  if constexpr (KIND == kMx8Exact) {
+    if (__builtin_expect(__ballot(far) != 0, 0))
+      far_sums(a, m0, (int64_t)a.rows - 1, n0, r16, g, acc, [](int, int) { return f32x4v{0, 0, 0, 0}; },
+               [&](auto tile) __attribute__((always_inline)) {
+#pragma clang loop unroll(disable)
+                 for (int kt0 = wave * kBatch; kt0 < a.k_tiles; kt0 += kWaves * kBatch)
+#pragma clang loop unroll(disable)
+                   for (int kt = kt0; kt < min(kt0 + kBatch, a.k_tiles); ++kt) tile(kt);
+               });
   }
 #pragma unroll
   for (int e = 0; e < MT; ++e)
