@@ -21,14 +21,22 @@ def _fp(a):
     return a.ctypes.data_as(POINTER(c_float)) if a is not None else None
 
 
+def _int32(v, what):
+    """v, where the C side takes 32 bits (ctypes would cut off the rest)."""
+    if not -0x80000000 <= v < 0x80000000:
+        raise ValueError("%s: %d does not fit 32 bits" % (what, v))
+    return v
+
+
 def _rows(a, cols, what):
     """A float32 [T x cols] array with contiguous rows, and its row stride in elements."""
     a = np.asarray(a, dtype=np.float32)
     if a.ndim != 2 or a.shape[1] != cols:
         raise ValueError("%s: shape %s, %d columns expected" % (what, a.shape, cols))
-    if a.strides[1] != 4 or a.strides[0] % 4 or a.strides[0] < 4 * cols:
+    _int32(a.shape[0], what)
+    if a.strides[1] != 4 or a.strides[0] % 4 or not 4 * cols <= a.strides[0] < 4 * 0x80000000:
         a = np.ascontiguousarray(a)
-    return a, max(a.strides[0] // 4, cols)
+    return a, a.strides[0] // 4 if a.shape[0] > 1 else cols
 
 
 class Matrix:
@@ -36,6 +44,8 @@ class Matrix:
     the scales' address and row stride in bytes (struct amlike_matrix).  Keeps no memory alive."""
 
     def __init__(self, ptr, type, ld, scales_ptr=0, ld_scales=0):
+        if not (0 <= ptr < 1 << 64 and 0 <= scales_ptr < 1 << 64 and -1 << 63 <= ld < 1 << 63 and -1 << 63 <= ld_scales < 1 << 63):
+            raise ValueError("Matrix: address or row stride out of range")
         self.c = _lib.Matrix(ptr, scales_ptr, ld, ld_scales, TYPES[type])
         self.ref = byref(self.c)
 
@@ -46,6 +56,8 @@ def _ref(m):
 
 def ConvertDevice(x, rows, cols, out, stream=None):
     """out = x in out's type (amlike_convert_dev); x and out are Matrix."""
+    if not (-0x80000000 <= rows < 0x80000000 and -0x80000000 <= cols < 0x80000000):
+        _int32(rows, "rows"), _int32(cols, "cols")
     rc = _lib.lib().amlike_convert_dev(x.ref, rows, cols, out.ref, stream)
     if rc:
         _lib.check(rc)
@@ -56,6 +68,7 @@ class RmsNorm:
 
     def __init__(self, dim, weight=None, eps=1e-5, device=None):
         L = _lib.lib()
+        _int32(int(dim), "dim")
         if device is not None:
             _lib.check(L.amlike_init(int(device)))
         w = None if weight is None else np.ascontiguousarray(weight, np.float32)
@@ -93,6 +106,8 @@ class RmsNorm:
 
     def ApplyDevice(self, x, rows, out, residual=None, sum=None, stream=None):
         """Matrix arguments, asynchronous on `stream` (amlike_norm_apply_dev)."""
+        if not -0x80000000 <= rows < 0x80000000:
+            _int32(rows, "rows")
         rc = self._apply(self._h, x.ref, _ref(residual), rows, _ref(sum), out.ref, stream)
         if rc:
             _lib.check(rc)
@@ -108,7 +123,7 @@ class Linear:
         w = np.asarray(weights, np.float32)
         if w.ndim != 2:
             raise ValueError("weights of %s" % (w.shape,))
-        w, ld = _rows(w, w.shape[1], "weights")
+        w, ld = _rows(w, _int32(w.shape[1], "weights"), "weights")
         b = None if bias is None else np.ascontiguousarray(bias, np.float32)
         if b is not None and b.shape != (w.shape[0],):
             raise ValueError("bias of %s for %d outputs" % (b.shape, w.shape[0]))
@@ -147,6 +162,8 @@ class Linear:
 
     def ApplyDevice(self, x, rows, out, activation="none", residual=None, stream=None):
         """Matrix arguments, asynchronous on `stream` (amlike_linear_apply_dev)."""
+        if not -0x80000000 <= rows < 0x80000000:
+            _int32(rows, "rows")
         rc = self._apply(self._h, x.ref, rows, ACTIVATIONS[activation], _ref(residual), out.ref, stream)
         if rc:
             _lib.check(rc)

@@ -89,3 +89,27 @@ def test_the_reference_of_the_8_bit_form():
     assert torch.equal(U.from_mx8(q, s), x) and (s == 127).all()
     for top, k in ((448.0, 0), (448.0001, 1), (224.0, -1), (1.75, -8), (1.7501, -7), (2.0 ** 127, 119), (0.0, -127), (2.0 ** -149, -127)):
         assert int(U.mx8_exponents(torch.full((1, 32), top, dtype=torch.float64))[0, 0]) == k
+
+
+@pytest.mark.parametrize("big", [2 ** 31, 2 ** 32 + 3, -2 ** 31 - 1, 2 ** 40])
+def test_python_mirror_refuses_counts_that_leave_32_bits(big):
+    """Beyond 32 bits ctypes would pass on what is left of them: 2^32 + 3 rows would be 3."""
+    x, out = dense.Matrix(4096, "bf16", 64), dense.Matrix(1 << 20, "f32", 64)
+    for rows, cols in ((big, 64), (4, big)):
+        with pytest.raises(ValueError):
+            dense.ConvertDevice(x, rows, cols, out)
+    with pytest.raises(ValueError):
+        dense.RmsNorm(big)
+    for cls in (dense.RmsNorm, dense.Linear):  # (the check comes before the handle is looked at)
+        h = cls.__new__(cls)
+        with pytest.raises(ValueError):
+            h.ApplyDevice(x, big, out)
+    wide = np.lib.stride_tricks.as_strided(np.zeros(2, np.float32), shape=(1, 2), strides=(4 * (2 ** 32 + 2), 4))
+    a, ld = dense._rows(wide, 2, "x")  # a stride too large for the C side is copied away
+    assert ld == 2 and a.flags.c_contiguous
+
+
+def test_python_mirror_refuses_strides_that_leave_64_bits():
+    for kw in (dict(ld=2 ** 63), dict(ld=2 ** 64 + 64), dict(ld=64, ld_scales=2 ** 64 + 2), dict(ptr=2 ** 64 + 4096, ld=64), dict(ptr=-1, ld=64)):
+        with pytest.raises(ValueError):
+            dense.Matrix(kw.pop("ptr", 4096), "mx8", kw.pop("ld"), 1 << 20, kw.pop("ld_scales", 2))
