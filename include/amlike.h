@@ -260,7 +260,10 @@ enum amlike_type {
  * of (r, c) is scales[r * ld_scales + c / 32].  Any ld >= the columns, any ld_scales >=
  * ceil(columns / 32); what lies behind a row's columns and behind the last row is neither
  * needed nor written.  Rows (of scales too) that start on 16 bytes, and for amlike_linear's x hold a
- * multiple of 16 bytes, are the fast case. */
+ * multiple of 16 bytes, are the fast case.
+ * Matrices must not overlap where a call says so: no byte may belong to both.  They may lie side by side
+ * in the rows of one buffer, or take its rows in turn; in such a stretch they are refused if their rows
+ * meet modulo the greatest common divisor of their row strides. */
 typedef struct amlike_matrix {
   void *data;
   void *scales; /* AMLIKE_MX8 only, else NULL */

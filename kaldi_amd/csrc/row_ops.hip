@@ -10,6 +10,7 @@
 #include <cmath>
 #include <mutex>
 #include <new>
+#include <numeric>
 
 #include "dense_common.h"
 
@@ -215,16 +216,27 @@ int CheckMatrix(const char *call, const char *name, const amlike_matrix_t *m, in
 
 namespace {
 
-struct Extent {
-  uintptr_t lo, hi;
+// Rows of bytes: the values or the scales of a matrix.  (A single row has no stride.)
+struct Strip {
+  uintptr_t at;
+  uint64_t stride, width, rows;
 };
-int Extents(const amlike_matrix_t *m, int64_t rows, int64_t cols, Extent e[2]) {
-  const uintptr_t p = reinterpret_cast<uintptr_t>(m->data);
-  e[0] = {p, p + ((uintptr_t)(rows - 1) * m->ld + cols) * TypeBytes(m->type)};
+int Strips(const amlike_matrix_t *m, int64_t rows, int64_t cols, Strip s[2]) {
+  const uint64_t es = TypeBytes(m->type), n = (uint64_t)rows;
+  s[0] = {reinterpret_cast<uintptr_t>(m->data), n > 1 ? (uint64_t)m->ld * es : 0, (uint64_t)cols * es, n};
   if (m->type != AMLIKE_MX8) return 1;
-  const uintptr_t s = reinterpret_cast<uintptr_t>(m->scales);
-  e[1] = {s, s + (uintptr_t)(rows - 1) * m->ld_scales + (cols + 31) / 32};
+  s[1] = {reinterpret_cast<uintptr_t>(m->scales), n > 1 ? (uint64_t)m->ld_scales : 0, (uint64_t)(cols + 31) / 32, n};
   return 2;
+}
+// Whether the bytes from first to last meet, and modulo the strides' greatest common divisor too:
+// matrices side by side in one buffer, or in its rows in turn, do not.
+bool StripsMeet(const Strip &a, const Strip &b) {
+  const uintptr_t a_end = a.at + (a.rows - 1) * a.stride + a.width, b_end = b.at + (b.rows - 1) * b.stride + b.width;
+  if (a.at >= b_end || b.at >= a_end) return false;
+  const uint64_t g = std::gcd(a.stride, b.stride);
+  if (g == 0) return true;  // two single rows
+  const uint64_t d = b.at >= a.at ? (b.at - a.at) % g : (g - (a.at - b.at) % g) % g;
+  return d < a.width || d + b.width > g;
 }
 
 template <int TIN, bool NORM, int TPR, int NCH>
@@ -279,11 +291,11 @@ constexpr int kNormMaxDim = 32768;  // 1024 threads x 4 chunks x 8 columns
 
 bool MatricesOverlap(const amlike_matrix_t *a, int64_t rows_a, int64_t cols_a, const amlike_matrix_t *b,
                      int64_t rows_b, int64_t cols_b) {
-  Extent ea[2], eb[2];
-  const int na = Extents(a, rows_a, cols_a, ea), nb = Extents(b, rows_b, cols_b, eb);
+  Strip sa[2], sb[2];
+  const int na = Strips(a, rows_a, cols_a, sa), nb = Strips(b, rows_b, cols_b, sb);
   for (int i = 0; i < na; ++i)
     for (int j = 0; j < nb; ++j)
-      if (ea[i].lo < eb[j].hi && eb[j].lo < ea[i].hi) return true;
+      if (StripsMeet(sa[i], sb[j])) return true;
   return false;
 }
 

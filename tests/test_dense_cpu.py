@@ -113,3 +113,30 @@ def test_python_mirror_refuses_strides_that_leave_64_bits():
     for kw in (dict(ld=2 ** 63), dict(ld=2 ** 64 + 64), dict(ld=64, ld_scales=2 ** 64 + 2), dict(ptr=2 ** 64 + 4096, ld=64), dict(ptr=-1, ld=64)):
         with pytest.raises(ValueError):
             dense.Matrix(kw.pop("ptr", 4096), "mx8", kw.pop("ld"), 1 << 20, kw.pop("ld_scales", 2))
+
+
+# (two matrices of 4 x 64 bf16 in a stretch of memory, and how they lie)
+APART = [(dict(ld=128), dict(ptr=4096 + 128, ld=128)),                                 # side by side
+         (dict(ptr=4096 + 128, ld=128), dict(ld=128)),
+         (dict(ld=192), dict(ptr=4096 + 128, type_="f32", ld=96)),                     # 128 and 256 bytes of 384
+         (dict(ld=128), dict(ptr=4096 + 128, ld=256)),                                 # every second row's second half
+         (dict(ld=128), dict(ptr=4096 + 3 * 256 + 128, ld=64)),                        # behind the last row
+         (dict(ld=128), dict(ptr=4096 + 128, type_="mx8", ld=256, scales=4096 + 192, ld_scales=256))]
+MEETING = [(dict(ld=128), dict(ptr=4096 + 126, ld=128)), (dict(ptr=4096 + 126, ld=128), dict(ld=128)),
+           (dict(ld=128), dict(ptr=4096 + 130, ld=128)), (dict(ld=128), dict(ptr=4096 + 128, ld=64)),
+           (dict(ld=128), dict(ptr=4096 + 3 * 256 + 126, ld=64)), (dict(ld=128), dict(ptr=4096 + 128, type_="f32", ld=64)),
+           (dict(ld=128), dict(ptr=4096 + 128, type_="mx8", ld=256, scales=4096 + 255, ld_scales=256))]
+
+
+@pytest.mark.parametrize("x,out", MEETING)
+def test_matrices_that_share_bytes_are_refused(x, out):
+    assert convert(matrix(**x), 4, 64, matrix(**out)) == _lib.EINVAL
+    assert "overlap" in _lib.lib().amlike_last_error().decode()
+
+
+@pytest.mark.parametrize("x,out", APART)
+def test_matrices_side_by_side_are_not_refused(x, out):
+    """Without a GPU the call ends where it looks for one, behind the checks."""
+    if _lib.lib().amlike_device_count() > 0:
+        pytest.skip("the addresses are made up")
+    assert convert(matrix(**x), 4, 64, matrix(**out)) == _lib.ENODEV

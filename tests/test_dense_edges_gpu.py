@@ -24,3 +24,72 @@ def test_silu_of_large_negative_arguments(amlike_device, rows, tout):
     torch.cuda.synchronize()
     want = x / (1 + torch.exp(-x))
     U.check_output(out, want, (6 + 2 * x.abs().clamp(max=200)) * 2.0 ** -23 * want.abs())
+
+
+class Slices:
+    """Column blocks of one bf16 buffer whose first and last columns are guards."""
+
+    def __init__(self, rows, widths, seed):
+        self.rows, self.widths = rows, widths
+        self.at = [8 + sum(widths[:i]) for i in range(len(widths))]
+        ld = 16 + sum(widths)
+        self.buf = torch.randn((rows, ld), generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+        self.start = self.buf.clone()
+        self.m = [dense.Matrix(self.buf.data_ptr() + 2 * a, "bf16", ld) for a in self.at]
+
+    def block(self, i, before=False):
+        return (self.start if before else self.buf)[:, self.at[i]:self.at[i] + self.widths[i]].cpu().double()
+
+    def assert_only(self, *written):
+        keep = torch.ones(self.buf.shape[1], dtype=torch.bool)
+        for i in written:
+            keep[self.at[i]:self.at[i] + self.widths[i]] = False
+        assert torch.equal(self.buf[:, keep.cuda()], self.start[:, keep.cuda()])
+
+
+@pytest.mark.parametrize("rows", [3, 70, 500])
+def test_operands_and_results_side_by_side_in_one_buffer(amlike_device, rows):
+    """x, residual, sum and output as column blocks of one wide buffer: the same bits as apart."""
+    s = Slices(rows, [200, 200, 200, 200], 1)
+    norm = dense.RmsNorm(200)
+    norm.ApplyDevice(s.m[0], rows, s.m[3], residual=s.m[1], sum=s.m[2])
+    apart = [U.DeviceMatrix(rows, 200, "bf16", fill=s.block(i, True)) for i in range(4)]
+    norm.ApplyDevice(apart[0].m, rows, apart[3].m, residual=apart[1].m, sum=apart[2].m)
+    torch.cuda.synchronize()
+    s.assert_only(2, 3)
+    assert torch.equal(s.block(2), apart[2].values()) and torch.equal(s.block(3), apart[3].values())
+
+    s = Slices(rows, [360, 264, 264], 2)
+    lin = dense.Linear(torch.randn((264, 360), generator=torch.Generator().manual_seed(3)).numpy(), None, "bf16")
+    lin.ApplyDevice(s.m[0], rows, s.m[1], residual=s.m[2])
+    apart = [U.DeviceMatrix(rows, s.widths[i], "bf16", 8, fill=s.block(i, True)) for i in range(3)]
+    lin.ApplyDevice(apart[0].m, rows, apart[1].m, residual=apart[2].m)
+    torch.cuda.synchronize()
+    s.assert_only(1)
+    assert torch.equal(s.block(1), apart[1].values())
+
+    s = Slices(rows, [64, 64], 4)
+    dense.ConvertDevice(s.m[0], rows, 64, s.m[1])
+    torch.cuda.synchronize()
+    s.assert_only(1)
+    assert torch.equal(s.block(1), s.block(0, True))
+
+
+def test_an_8_bit_layer_between_rows_of_one_buffer(amlike_device):
+    """Rows of [x | scales of x | output | scales of the output]: a layer in place in its record."""
+    rows, k, n = 130, 256, 512
+    x = U.rounded(torch.randn((rows, k), generator=torch.Generator().manual_seed(5)).double(), "mx8")
+    w = torch.randn((n, k), generator=torch.Generator().manual_seed(6)).numpy()
+    lin = dense.Linear(w, None, "mx8")
+    apart, out = U.DeviceMatrix(rows, k, "mx8", 16, fill=x), U.DeviceMatrix(rows, n, "mx8", 16)
+    lin.ApplyDevice(apart.m, rows, out.m, activation="relu")
+    ld = k + 16 + n + 16
+    buf = torch.zeros((rows, ld), dtype=torch.uint8, device="cuda")
+    buf[:, :k] = apart.buf[:rows, :k]
+    buf[:, k:k + 8] = apart.scales[:rows, :8]
+    p = buf.data_ptr()
+    lin.ApplyDevice(dense.Matrix(p, "mx8", ld, p + k, ld), rows, dense.Matrix(p + k + 16, "mx8", ld, p + k + 16 + n, ld), activation="relu")
+    torch.cuda.synchronize()
+    assert torch.equal(buf[:, k + 16:k + 16 + n], out.buf[:rows, :n])
+    assert torch.equal(buf[:, k + 16 + n:], out.scales[:rows, :16])
+    assert torch.equal(buf[:, :k], apart.buf[:rows, :k]) and (buf[:, k + 8:k + 16] == 0).all()
