@@ -262,8 +262,7 @@ enum amlike_type {
  * needed nor written.  Rows (of scales too) that start on 16 bytes, and for amlike_linear's x hold a
  * multiple of 16 bytes, are the fast case.
  * Matrices must not overlap where a call says so: no byte may belong to both.  They may lie side by side
- * in the rows of one buffer, or take its rows in turn; in such a stretch they are refused if their rows
- * meet modulo the greatest common divisor of their row strides. */
+ * in the rows of one buffer, or take its rows in turn. */
 typedef struct amlike_matrix {
   void *data;
   void *scales; /* AMLIKE_MX8 only, else NULL */

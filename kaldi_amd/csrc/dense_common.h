@@ -13,8 +13,7 @@ static inline int TypeBytes(int type) { return type == AMLIKE_F32 ? 4 : type == 
 // AMLIKE_OK or AMLIKE_EINVAL with a text: `m` describes a [rows x cols] matrix that a kernel may
 // touch.  With rows == 0 only the type is looked at.
 int CheckMatrix(const char *call, const char *name, const amlike_matrix_t *m, int64_t rows, int64_t cols);
-// Whether the bytes of two matrices (values or scales) meet.  Matrices that share a stretch of memory are
-// taken as apart where their rows are, modulo the greatest common divisor of the row strides.
+// Whether a byte (of values or scales) belongs to both matrices.
 bool MatricesOverlap(const amlike_matrix_t *a, int64_t rows_a, int64_t cols_a, const amlike_matrix_t *b,
                      int64_t rows_b, int64_t cols_b);
 // Whether they are one matrix: an element is read and written by the same thread then.

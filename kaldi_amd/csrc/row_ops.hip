@@ -10,7 +10,7 @@
 #include <cmath>
 #include <mutex>
 #include <new>
-#include <numeric>
+#include <utility>
 
 #include "dense_common.h"
 
@@ -228,15 +228,38 @@ int Strips(const amlike_matrix_t *m, int64_t rows, int64_t cols, Strip s[2]) {
   s[1] = {reinterpret_cast<uintptr_t>(m->scales), n > 1 ? (uint64_t)m->ld_scales : 0, (uint64_t)(cols + 31) / 32, n};
   return 2;
 }
-// Whether the bytes from first to last meet, and modulo the strides' greatest common divisor too:
-// matrices side by side in one buffer, or in its rows in turn, do not.
-bool StripsMeet(const Strip &a, const Strip &b) {
+// The sum of floor((a i + b) / m) over 0 <= i < n, by turning the count of lattice points below the line
+// round as often as Euclid's algorithm has steps.
+typedef unsigned __int128 Wide;
+Wide FloorSum(Wide n, Wide m, Wide a, Wide b) {
+  Wide sum = 0;
+  for (;;) {
+    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const Wide top = a * n + b;
+    if (top < m) return sum;
+    n = top / m;
+    b = top % m;
+    std::swap(m, a);
+  }
+}
+// Whether a byte belongs to both.
+bool StripsMeet(Strip a, Strip b) {
+  if (b.stride == 0) std::swap(a, b);
   const uintptr_t a_end = a.at + (a.rows - 1) * a.stride + a.width, b_end = b.at + (b.rows - 1) * b.stride + b.width;
   if (a.at >= b_end || b.at >= a_end) return false;
-  const uint64_t g = std::gcd(a.stride, b.stride);
-  if (g == 0) return true;  // two single rows
-  const uint64_t d = b.at >= a.at ? (b.at - a.at) % g : (g - (a.at - b.at) % g) % g;
-  return d < a.width || d + b.width > g;
+  if (b.stride == 0) return true;  // two single rows
+  // Rows of a that lie within b's stretch, if only in part.  A row meets a row of b, whichever, if one of the
+  // starts b.at + j * b.stride lies in the b.width - 1 bytes before it or in itself: the floors count them.
+  // (A start that is not one of b's, before the first or behind the last, only counts where the first or last does.)
+  const uint64_t lo = a.at + a.width > b.at ? 0 : a.stride ? (b.at - (a.at + a.width)) / a.stride + 1 : a.rows;
+  const uint64_t hi = a.stride ? std::min<uint64_t>(a.rows - 1, (b_end - 1 - a.at) / a.stride) : 0;
+  if (lo > hi) return false;
+  const uint64_t up = (b.at + b.width) / b.stride + 1;  // (the starts moved up by whole strides: nothing is negative)
+  const Wide first = (Wide)a.at + (Wide)lo * a.stride + (Wide)up * b.stride - b.at;
+  const Wide n = hi - lo + 1;
+  return FloorSum(n, b.stride, a.stride, first + a.width - 1) != FloorSum(n, b.stride, a.stride, first - b.width);
 }
 
 template <int TIN, bool NORM, int TPR, int NCH>

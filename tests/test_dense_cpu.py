@@ -140,3 +140,43 @@ def test_matrices_side_by_side_are_not_refused(x, out):
     if _lib.lib().amlike_device_count() > 0:
         pytest.skip("the addresses are made up")
     assert convert(matrix(**x), 4, 64, matrix(**out)) == _lib.ENODEV
+
+
+def test_overlap_is_exact():
+    """Small matrices in a small stretch of memory against the sets of their bytes."""
+    if _lib.lib().amlike_device_count() > 0:
+        pytest.skip("the addresses are made up")
+    rng = np.random.default_rng(1)
+    sizes = {"f32": 4, "bf16": 2, "f16": 2, "mx8": 1}
+    met = 0
+    for _ in range(6000):
+        rows, cols = int(rng.integers(1, 12)), int(rng.integers(1, 40))
+        bytes_, args = [], []
+        for t in (["f32", "bf16", "f16"][rng.integers(3)], list(sizes)[rng.integers(4)]):
+            at, ld = 4096 + 4 * int(rng.integers(0, 300)), cols + int(rng.integers(0, 4)) * int(rng.integers(0, 60))
+            groups = (cols + 31) // 32
+            scales, ld_scales = 4096 + int(rng.integers(0, 1200)) if t == "mx8" else 0, groups + int(rng.integers(0, 80))
+            mine = {at + (r * ld + c) * sizes[t] + i for r in range(rows) for c in range(cols) for i in range(sizes[t])}
+            if t == "mx8":
+                own = {scales + r * ld_scales + c for r in range(rows) for c in range(groups)}
+                while mine & own:  # (its scales lie elsewhere)
+                    scales += 1 << 20
+                    own = {v + (1 << 20) for v in own}
+                mine |= own
+            bytes_.append(mine)
+            args.append(matrix(ptr=at, type_=t, ld=ld, scales=scales, ld_scales=ld_scales))
+        meet = bool(bytes_[0] & bytes_[1])
+        met += meet
+        assert convert(args[0], rows, cols, args[1]) == (_lib.EINVAL if meet else _lib.ENODEV)
+    assert 1000 < met < 5000  # both happen
+
+
+def test_overlap_of_matrices_as_large_as_there_are():
+    """2^31 - 1 rows whose strides share no divisor: refused or not within no time."""
+    if _lib.lib().amlike_device_count() > 0:
+        pytest.skip("the addresses are made up")
+    rows = 2 ** 31 - 1
+    for ld, at, meet in ((100003, 2 * 100003 * rows - 16, False), (100003, 2 * 100003 * (rows - 1) + 14, True), (100001, 0, True),
+                         (100003, 16, False), (100003, 14, True), (100003, 2 * 100003 - 16, False), (100003, 2 * 100003 - 14, True)):
+        a, b = matrix(ptr=4096, ld=100003), matrix(ptr=4096 + at, ld=ld)
+        assert convert(a, rows, 8, b) == (_lib.EINVAL if meet else _lib.ENODEV), (ld, at)
