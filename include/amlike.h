@@ -262,7 +262,8 @@ enum amlike_type {
  * needed nor written.  Rows (of scales too) that start on 16 bytes, and for amlike_linear's x hold a
  * multiple of 16 bytes, are the fast case.
  * Matrices must not overlap where a call says so: no byte may belong to both.  They may lie side by side
- * in the rows of one buffer, or take its rows in turn. */
+ * in the rows of one buffer, or take its rows in turn.  The same holds for the values and the scales of
+ * a matrix that is written. */
 typedef struct amlike_matrix {
   void *data;
   void *scales; /* AMLIKE_MX8 only, else NULL */

@@ -13,6 +13,8 @@ static inline int TypeBytes(int type) { return type == AMLIKE_F32 ? 4 : type == 
 // AMLIKE_OK or AMLIKE_EINVAL with a text: `m` describes a [rows x cols] matrix that a kernel may
 // touch.  With rows == 0 only the type is looked at.
 int CheckMatrix(const char *call, const char *name, const amlike_matrix_t *m, int64_t rows, int64_t cols);
+// The same for a matrix that is written: its values and scales do not share bytes either.
+int CheckOutput(const char *call, const amlike_matrix_t *out, int64_t rows, int64_t cols);
 // Whether a byte (of values or scales) belongs to both matrices.
 bool MatricesOverlap(const amlike_matrix_t *a, int64_t rows_a, int64_t cols_a, const amlike_matrix_t *b,
                      int64_t rows_b, int64_t cols_b);

@@ -214,7 +214,7 @@ int amlike_linear_apply_dev(const amlike_linear_t *h, const amlike_matrix_t *x, 
     return AMLIKE_EINVAL;
   }
   if (int rc = CheckMatrix(call, "x", x, rows, h->k)) return rc;
-  if (int rc = CheckMatrix(call, "out", out, rows, h->n)) return rc;
+  if (int rc = CheckOutput(call, out, rows, h->n)) return rc;
   if (residual)
     if (int rc = CheckMatrix(call, "residual", residual, rows, h->n)) return rc;
   if (x->type != h->type || (residual && residual->type == AMLIKE_MX8)) {

@@ -322,6 +322,16 @@ bool MatricesOverlap(const amlike_matrix_t *a, int64_t rows_a, int64_t cols_a, c
   return false;
 }
 
+int CheckOutput(const char *call, const amlike_matrix_t *out, int64_t rows, int64_t cols) {
+  if (int rc = CheckMatrix(call, "out", out, rows, cols)) return rc;
+  Strip s[2];
+  if (rows > 0 && Strips(out, rows, cols, s) == 2 && StripsMeet(s[0], s[1])) {
+    SetError("%s: out's values and scales overlap", call);
+    return AMLIKE_EINVAL;
+  }
+  return AMLIKE_OK;
+}
+
 int LaunchConvert(const amlike_matrix_t &x, int64_t rows, int64_t cols, const amlike_matrix_t &out, hipStream_t st) {
   RowArgs a = {};
   a.x = x.data;
@@ -362,7 +372,7 @@ int amlike_convert_dev(const amlike_matrix_t *x, int32_t rows, int32_t cols, con
     return AMLIKE_EINVAL;
   }
   if (int rc = CheckMatrix(call, "x", x, rows, cols)) return rc;
-  if (int rc = CheckMatrix(call, "out", out, rows, cols)) return rc;
+  if (int rc = CheckOutput(call, out, rows, cols)) return rc;
   if (x->type == AMLIKE_MX8) {
     SetError("%s: x in 8 bits is not an input", call);
     return AMLIKE_EINVAL;
@@ -436,7 +446,7 @@ int amlike_norm_apply_dev(const amlike_norm_t *h, const amlike_matrix_t *x, cons
   }
   const int dim = h->dim;
   if (int rc = CheckMatrix(call, "x", x, rows, dim)) return rc;
-  if (int rc = CheckMatrix(call, "out", out, rows, dim)) return rc;
+  if (int rc = CheckOutput(call, out, rows, dim)) return rc;
   if (residual)
     if (int rc = CheckMatrix(call, "residual", residual, rows, dim)) return rc;
   if (sum)

@@ -180,3 +180,26 @@ def test_overlap_of_matrices_as_large_as_there_are():
                          (100003, 16, False), (100003, 14, True), (100003, 2 * 100003 - 16, False), (100003, 2 * 100003 - 14, True)):
         a, b = matrix(ptr=4096, ld=100003), matrix(ptr=4096 + at, ld=ld)
         assert convert(a, rows, 8, b) == (_lib.EINVAL if meet else _lib.ENODEV), (ld, at)
+
+
+@pytest.mark.parametrize("scales,ld_scales", [(4096, 4), (4096 + 62, 4), (4096 + 3 * 128 + 63, 1 << 20), (4096 + 63, 128), (4096 - 1, 4)])
+def test_values_and_scales_of_an_output_that_share_bytes_are_refused(scales, ld_scales):
+    """(Which of a value and a scale was written last would be anybody's guess.)"""
+    x = matrix(ptr=1 << 20)
+    assert convert(x, 4, 64, matrix(ptr=4096, type_="mx8", ld=128, scales=scales, ld_scales=ld_scales)) == _lib.EINVAL
+    assert "scales overlap" in _lib.lib().amlike_last_error().decode()
+    # bytes [4096, 4160) and two scales
+    assert convert(x, 1, 64, matrix(ptr=4096, type_="mx8", ld=64, scales=4095, ld_scales=2)) == _lib.EINVAL
+    assert convert(x, 1, 64, matrix(ptr=4096, type_="mx8", ld=64, scales=4159, ld_scales=2)) == _lib.EINVAL
+
+
+@pytest.mark.parametrize("rows,scales,ld_scales", [(4, 4096 + 64, 4), (4, 4096 + 64, 128), (4, 4096 + 126, 128), (1, 4094, 2), (1, 4160, 2)])
+def test_scales_of_an_output_between_its_values_are_not_refused(rows, scales, ld_scales):
+    if _lib.lib().amlike_device_count() > 0:
+        pytest.skip("the addresses are made up")
+    out = matrix(ptr=4096, type_="mx8", ld=128, scales=scales, ld_scales=ld_scales)
+    assert convert(matrix(ptr=1 << 20), rows, 64, out) == _lib.ENODEV
+
+
+def test_no_rows_are_no_overlap():
+    assert convert(matrix(ptr=1 << 20), 0, 64, matrix(ptr=4096, type_="mx8", ld=64, scales=4096, ld_scales=2)) == _lib.OK
