@@ -229,9 +229,11 @@ int amlike_linear_apply_dev(const amlike_linear_t *h, const amlike_matrix_t *x, 
   }
   LinearArgs a = {};
   a.x = static_cast<const uint8_t *>(x->data);
-  a.x_scales = static_cast<const uint8_t *>(x->scales);
   a.ldx = x->ld * TypeBytes(x->type);
-  a.ld_xs = x->ld_scales;
+  if (x->type == AMLIKE_MX8) {  // (in the other types the fields may hold anything)
+    a.x_scales = static_cast<const uint8_t *>(x->scales);
+    a.ld_xs = x->ld_scales;
+  }
   a.w = h->d_w;
   a.w_scales = h->d_scales;
   a.bias = h->d_bias;
@@ -242,9 +244,11 @@ int amlike_linear_apply_dev(const amlike_linear_t *h, const amlike_matrix_t *x, 
     a.res_type = residual->type;
   }
   a.out = out->data;
-  a.out_scales = static_cast<uint8_t *>(out->scales);
   a.ldo = out->ld;
-  a.ld_os = out->ld_scales;
+  if (out->type == AMLIKE_MX8) {
+    a.out_scales = static_cast<uint8_t *>(out->scales);
+    a.ld_os = out->ld_scales;
+  }
   a.out_type = out->type;
   a.rows = rows;
   a.k = h->k;

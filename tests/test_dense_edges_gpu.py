@@ -93,3 +93,23 @@ def test_an_8_bit_layer_between_rows_of_one_buffer(amlike_device):
     assert torch.equal(buf[:, k + 16:k + 16 + n], out.buf[:rows, :n])
     assert torch.equal(buf[:, k + 16 + n:], out.scales[:rows, :16])
     assert torch.equal(buf[:, :k], apart.buf[:rows, :k]) and (buf[:, k + 8:k + 16] == 0).all()
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16"])
+def test_what_a_16_bit_matrix_has_as_scales_is_not_looked_at(amlike_device, type_):
+    """scales and ld_scales belong to 8-bit matrices: left as anything, they change neither kernel nor bits."""
+    rows, k, n = 1024, 1000, 1000
+    lin = dense.Linear(torch.randn((n, k), generator=torch.Generator().manual_seed(7)).numpy(), None, type_)
+    x = U.DeviceMatrix(rows, k, type_, 8, fill=torch.randn((rows, k), generator=torch.Generator().manual_seed(8)).double())
+    r = U.DeviceMatrix(rows, n, "f32", 0, fill=torch.ones((rows, n), dtype=torch.float64))
+    want, out = U.DeviceMatrix(rows, n, "f32"), U.DeviceMatrix(rows, n, "f32")
+    lin.ApplyDevice(x.m, rows, want.m, residual=r.m)
+    odd = [dense.Matrix(m.buf.data_ptr(), m.type, m.ld, 4097, 2 ** 62 + 5) for m in (x, out, r)]
+    lin.ApplyDevice(odd[0], rows, odd[1], residual=odd[2])
+    torch.cuda.synchronize()
+    assert torch.equal(out.values(), want.values())
+    norm, y, z = dense.RmsNorm(k), U.DeviceMatrix(rows, k, "f32"), U.DeviceMatrix(rows, k, "f32")
+    norm.ApplyDevice(x.m, rows, y.m)
+    norm.ApplyDevice(odd[0], rows, dense.Matrix(z.buf.data_ptr(), "f32", z.ld, 4097, -3))
+    torch.cuda.synchronize()
+    assert torch.equal(y.values(), z.values())
