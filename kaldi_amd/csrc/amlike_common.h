@@ -17,6 +17,9 @@ namespace amlike {
 // Per-thread last error text (what KALDI_ERR would have printed).
 void SetError(const char *fmt, ...);
 const char *LastError();
+// The text of a HIP call's error, for SetError.  The error leaves HIP's own record, where the next check
+// of a launch, this library's or its caller's, would take it for its own.
+const char *HipFailure(hipError_t e);
 
 // Devices.  amlike_init(d) may be called for several devices (from one thread or from one
 // thread per device).  A handle lives on the device that was current for its creating thread:
@@ -148,7 +151,7 @@ static inline void SplitBf16x3(float x, uint16_t p[3]) {
   do {                                                                            \
     hipError_t e_ = (call);                                                       \
     if (e_ != hipSuccess) {                                                       \
-      amlike::SetError("%s failed: %s (%s:%d)", #call, hipGetErrorString(e_),     \
+      amlike::SetError("%s failed: %s (%s:%d)", #call, amlike::HipFailure(e_),    \
                        __FILE__, __LINE__);                                       \
       return (e_ == hipErrorOutOfMemory) ? AMLIKE_EOOM : AMLIKE_EHIP;             \
     }                                                                             \

@@ -26,6 +26,10 @@ void SetError(const char *fmt, ...) {
 }
 
 const char *LastError() { return g_err; }
+const char *HipFailure(hipError_t e) {
+  (void)hipGetLastError();
+  return hipGetErrorString(e);
+}
 int CurrentDevice() { return t_device >= 0 ? t_device : g_default_device.load(); }
 int NumComputeUnits() {
   int cur = -1;
@@ -59,7 +63,7 @@ int DeviceBuffer::Reserve(size_t want) {
   }
   if (e != hipSuccess) {
     ptr = nullptr;
-    SetError("hipMalloc of %zu bytes failed: %s", want, hipGetErrorString(e));
+    SetError("hipMalloc of %zu bytes failed: %s", want, HipFailure(e));
     return AMLIKE_EOOM;
   }
   bytes = grow;
@@ -333,7 +337,7 @@ int amlike_host_alloc(size_t bytes, void **ptr) {
   if (e != hipSuccess) {
     (void)hipGetLastError();
     *ptr = nullptr;
-    amlike::SetError("hipHostMalloc of %zu bytes failed: %s", bytes, hipGetErrorString(e));
+    amlike::SetError("hipHostMalloc of %zu bytes failed: %s", bytes, amlike::HipFailure(e));
     return AMLIKE_EOOM;
   }
   return AMLIKE_OK;

@@ -129,7 +129,7 @@ int amlike_xform_create(int32_t dim, int32_t left, int32_t right, const float *m
   }
   if (e == hipSuccess) e = hipStreamCreateWithFlags(&x->stream, hipStreamNonBlocking);
   if (e != hipSuccess) {
-    SetError("amlike_xform_create: %s", hipGetErrorString(e));
+    SetError("amlike_xform_create: %s", HipFailure(e));
     amlike_xform_destroy(x);
     return AMLIKE_EHIP;
   }

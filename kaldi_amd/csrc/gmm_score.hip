@@ -2591,7 +2591,7 @@ int amlike_gmm_create(const float *gconsts, const float *means_invvars, const fl
         e = hipMemcpy(g->d_offsets, pdf_offsets, (size_t)(num_pdfs + 1) * sizeof(int32_t),
                       hipMemcpyHostToDevice);
       if (e != hipSuccess) {
-        SetError("amlike_gmm_create: %s", hipGetErrorString(e));
+        SetError("amlike_gmm_create: %s", HipFailure(e));
         rc = AMLIKE_EHIP;
       }
     }
@@ -2602,7 +2602,7 @@ int amlike_gmm_create(const float *gconsts, const float *means_invvars, const fl
     if (e == hipSuccess) e = hipMemcpy(g->d_flag, &zero, sizeof(int), hipMemcpyHostToDevice);
     if (e == hipSuccess) e = hipStreamCreateWithFlags(&g->stream, hipStreamNonBlocking);
     if (e != hipSuccess) {
-      SetError("amlike_gmm_create: %s", hipGetErrorString(e));
+      SetError("amlike_gmm_create: %s", HipFailure(e));
       rc = AMLIKE_EHIP;
     }
   }

@@ -173,7 +173,7 @@ int amlike_linear_create(const float *weights, int32_t ld, const float *bias, in
   const hipError_t e = hipStreamCreateWithFlags(&h->stream, hipStreamNonBlocking);
   int rc = AMLIKE_OK;
   if (e != hipSuccess) {
-    SetError("amlike_linear_create: %s", hipGetErrorString(e));
+    SetError("amlike_linear_create: %s", HipFailure(e));
     rc = AMLIKE_EHIP;
   }
   if (rc == AMLIKE_OK) rc = PackWeights(h, weights, ld, bias);

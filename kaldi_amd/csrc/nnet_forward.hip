@@ -3693,7 +3693,7 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
             e = hipMemcpy(s.d_bias, bpad.data(), bpad.size() * sizeof(float), hipMemcpyHostToDevice);
         }
         if (e != hipSuccess) {
-          SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+          SetError("amlike_nnet_create: %s", HipFailure(e));
           rc = e == hipErrorOutOfMemory ? AMLIKE_EOOM : AMLIKE_EHIP;
         }
         break;
@@ -3735,7 +3735,7 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
                 e = hipMemcpy(a.d_wpr, rows_img.data(), rows_img.size() * sizeof(uint16_t), hipMemcpyHostToDevice);
             }
             if (e != hipSuccess) {
-              SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+              SetError("amlike_nnet_create: %s", HipFailure(e));
               rc = e == hipErrorOutOfMemory ? AMLIKE_EOOM : AMLIKE_EHIP;
             } else {
               a.fuse_gs = gs;
@@ -3760,7 +3760,7 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
         if (e == hipSuccess)
           e = hipMemcpy(s.d_begins, begins.data(), begins.size() * sizeof(int32_t), hipMemcpyHostToDevice);
         if (e != hipSuccess) {
-          SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+          SetError("amlike_nnet_create: %s", HipFailure(e));
           rc = AMLIKE_EHIP;
         }
         break;
@@ -3776,7 +3776,7 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
         if (e == hipSuccess)
           e = hipMemcpy(s.d_bias, c.bias, c.input_dim * sizeof(float), hipMemcpyHostToDevice);
         if (e != hipSuccess) {
-          SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+          SetError("amlike_nnet_create: %s", HipFailure(e));
           rc = AMLIKE_EHIP;
         }
         break;
@@ -3804,7 +3804,7 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
         if (e == hipSuccess)
           e = hipMemcpy(s.d_begins, src.data(), src.size() * sizeof(int32_t), hipMemcpyHostToDevice);
         if (e != hipSuccess) {
-          SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+          SetError("amlike_nnet_create: %s", HipFailure(e));
           rc = AMLIKE_EHIP;
         }
         break;
@@ -3857,7 +3857,7 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
       hipError_t e = hipMalloc(&a.d_wob, img.size() * sizeof(uint16_t));
       if (e == hipSuccess) e = hipMemcpy(a.d_wob, img.data(), img.size() * sizeof(uint16_t), hipMemcpyHostToDevice);
       if (e != hipSuccess) {
-        SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+        SetError("amlike_nnet_create: %s", HipFailure(e));
         rc = e == hipErrorOutOfMemory ? AMLIKE_EOOM : AMLIKE_EHIP;
       }
     }
@@ -3873,7 +3873,7 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
     if (e == hipSuccess)
       e = hipMemcpy(n->d_log_priors, lp.data(), lp.size() * sizeof(float), hipMemcpyHostToDevice);
     if (e != hipSuccess) {
-      SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+      SetError("amlike_nnet_create: %s", HipFailure(e));
       rc = AMLIKE_EHIP;
     }
     n->num_priors = num_priors;
@@ -3881,14 +3881,14 @@ int amlike_nnet_create(const amlike_component_t *comps, int32_t num, const float
   if (rc == AMLIKE_OK) {
     hipError_t e = hipMalloc(&n->d_flags, (n->stages.size() + 1) * sizeof(int));
     if (e != hipSuccess) {
-      SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+      SetError("amlike_nnet_create: %s", HipFailure(e));
       rc = AMLIKE_EHIP;
     }
   }
   if (rc == AMLIKE_OK) {
     hipError_t e = hipStreamCreateWithFlags(&n->stream, hipStreamNonBlocking);
     if (e != hipSuccess) {
-      SetError("amlike_nnet_create: %s", hipGetErrorString(e));
+      SetError("amlike_nnet_create: %s", HipFailure(e));
       rc = AMLIKE_EHIP;
     }
   }

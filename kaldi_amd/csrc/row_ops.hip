@@ -413,7 +413,7 @@ int amlike_norm_create(const float *weight, int32_t dim, float eps, amlike_norm_
   }
   if (e == hipSuccess) e = hipStreamCreateWithFlags(&h->stream, hipStreamNonBlocking);
   if (e != hipSuccess) {
-    SetError("amlike_norm_create: %s", hipGetErrorString(e));
+    SetError("amlike_norm_create: %s", HipFailure(e));
     amlike_norm_destroy(h);
     return e == hipErrorOutOfMemory ? AMLIKE_EOOM : AMLIKE_EHIP;
   }

@@ -1,10 +1,12 @@
 """The dense-layer operators at the ends of what they take, on the GPU."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import dense_util as U
-from kaldi_amd import dense
+from kaldi_amd import _lib, dense
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +115,30 @@ def test_what_a_16_bit_matrix_has_as_scales_is_not_looked_at(amlike_device, type
     norm.ApplyDevice(odd[0], rows, dense.Matrix(z.buf.data_ptr(), "f32", z.ld, 4097, -3))
     torch.cuda.synchronize()
     assert torch.equal(y.values(), z.values())
+
+
+def test_a_refusal_for_memory_leaves_no_error_behind(amlike_device):
+    """4 TB of weights, and host rows of 2^48 bytes: refused before the arrays are looked at; neither this library's
+    nor anybody else's next call finds the error."""
+    L, w, h = _lib.lib(), np.ones(8, np.float32), ctypes.c_void_p()
+    fp = w.ctypes.data_as(ctypes.POINTER(ctypes.c_float))
+    x, out = U.DeviceMatrix(4, 64, "f32", fill=torch.ones(4, 64)), U.DeviceMatrix(4, 64, "bf16")
+    norm = dense.RmsNorm(32768)
+    lin = dense.Linear(np.ones((32768, 32), np.float32), None, "bf16")
+    torch.cuda.synchronize()
+
+    def too_much():
+        assert L.amlike_linear_create(fp, 1 << 20, None, 1 << 20, 1 << 20, 1, ctypes.byref(h)) == _lib.EOOM and not h.value
+        yield
+        assert L.amlike_norm_apply(norm._h, fp, 32768, None, 0, 2 ** 31 - 1, None, 0, fp, 32768) == _lib.EOOM
+        yield
+        assert L.amlike_linear_apply(lin._h, fp, 32, 2 ** 31 - 1, 0, None, 0, fp, 32768) == _lib.EOOM
+        yield
+
+    for _ in too_much():
+        assert "out of memory" in L.amlike_last_error().decode()
+        assert L.amlike_convert_dev(x.m.ref, 4, 64, out.m.ref, None) == _lib.OK
+    for _ in too_much():
+        assert float(torch.ones(5, device="cuda").sum()) == 5.0
+    torch.cuda.synchronize()
+    assert (out.values() == 1).all()
