@@ -333,6 +333,12 @@ int32_t amlike_linear_device(const amlike_linear_t *linear);
 int amlike_linear_apply_dev(const amlike_linear_t *linear, const amlike_matrix_t *x, int32_t rows,
                             int32_t activation, const amlike_matrix_t *residual,
                             const amlike_matrix_t *out, void *stream);
+/* The kernel and its form that such a call takes on a device of `units` compute units (aligned: rows of x,
+ * and of its scales, start on 16 bytes and hold a multiple of 16), with the rows and outputs of a block's
+ * tile, tiles and blocks; needs no GPU.  "" for arguments out of range.  The text stays until the
+ * thread's next call. */
+const char *amlike_linear_kernel_info(int32_t type, int32_t out_type, int32_t rows, int32_t input_dim,
+                                      int32_t output_dim, int32_t aligned, int32_t units);
 /* Host pointers, fp32, synchronous: x is converted to the handle's type on the device. */
 int amlike_linear_apply(amlike_linear_t *linear, const float *x, int32_t ld, int32_t rows,
                         int32_t activation, const float *residual, int32_t ldr, float *out, int32_t ldo);

@@ -92,6 +92,7 @@ def _declare(lib):
         "amlike_linear_type": (c_int32, [c_void_p]),
         "amlike_linear_device": (c_int32, [c_void_p]),
         "amlike_linear_apply_dev": (ctypes.c_int, [c_void_p, mp, c_int32, c_int32, mp, mp, c_void_p]),
+        "amlike_linear_kernel_info": (c_char_p, [c_int32] * 7),
         "amlike_linear_apply": (ctypes.c_int, [c_void_p, fp, c_int32, c_int32, c_int32, fp, c_int32, fp, c_int32]),
         "amlike_nnet_create": (ctypes.c_int, [POINTER(Component), c_int32, fp, c_int32, POINTER(c_void_p)]),
         "amlike_nnet_destroy": (ctypes.c_int, [c_void_p]),

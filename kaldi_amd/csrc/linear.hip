@@ -1,5 +1,9 @@
 // amlike_linear_*: the host side of the matrix product with bias, activation and residual, and the
 // packing of its weights.  The kernels: linear_kernels.h.
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <cstdlib>
 #include <mutex>
 #include <new>
 
@@ -8,11 +12,64 @@
 namespace amlike {
 
 constexpr int kLinearMaxDim = 1 << 20;  // either dimension of a layer
+constexpr int kMaxBlocks = 1 << 22;     // of a launch
 
 extern template int LaunchLinear<AMLIKE_BF16>(const LinearArgs &, hipStream_t);
 extern template int LaunchLinear<AMLIKE_F16>(const LinearArgs &, hipStream_t);
 extern template int LaunchLinear<AMLIKE_MX8>(const LinearArgs &, hipStream_t);
 extern template int LaunchLinear<kMx8Exact>(const LinearArgs &, hipStream_t);
+
+// ---- the choice of a form ---------------------------------------------------------------------------------
+
+// The form with the least estimated time, from the turns that the busiest compute unit has to take.
+// Microseconds per k-tile and per turn, measured in bf16 at the sizes behind each line (less the
+// 2.2 that every launch takes); only their relation matters.
+//   256 x 256, 8 waves                      1.62 kt + 7    35554 x 2000 x 8600: 1118 (measured 1157)
+//   128 x 128, 4 waves, alone on its unit   0.65 kt + 2    1024 x 4096 x 4096: 44 (44.5)
+//              two of them                  0.95 kt + 4    4096 x 2048 x 2048: 34 (34.4)
+//   128 x 128, 2 groups of 4 waves          0.55 kt + 3    1024 x 4096 x 4096: 38 (38.7)
+//   64 x 64, 4 waves, alone                 0.31 kt + 1    300 x 360 x 2000: 2.9 (5.5 with the launch)
+//            two of them                    0.38 kt + 2    1024 x 4096 x 4096: 53 (54)
+//   64 x 64, 2 groups of 4 waves            0.27 kt + 1.5  32 x 4096 x 16384: 21 (22.4 with it)
+// Rows of x that do not start and end on 16 bytes go through registers, in two forms:
+//   64 x 64, four blocks a unit             0.36 kt each   1237 x 1999 x 2001 bf16: 30.0 (128 x 128: 39.5)
+//            alone                          0.45 kt        64 x 2000 x 1024: 14.4 (16.0 with it)
+//   128 x 128, alone / two of them   1.25 kt / 2.0 kt      2000 x 2002 x 4096 mx8: 32.0 (64 x 64: 53.1)
+// The thin kernel, whatever the rows' places; the second figure where they are not on 16 bytes
+// (sizes and times as above, all with the launch), and 0.5 a turn:
+//   16 rows x 16 outputs                    0.12, 0.18 kt  64 x 4096 x 1024: 9.5 (64 x 64: 21.3)
+//   16 rows x 32 outputs                    0.19, 0.20 kt  16 x 8192 x 8192: 24.9 (16 x 16: 31.1)
+//   32 rows x 16 outputs                    0.18, 0.33 kt  128 x 4096 x 1024: 13.0 (64 x 64: 21.4)
+//   32 rows x 32 outputs                    0.25, 0.37 kt  64 x 4096 x 4096: 17.5 (64 x 64: 21.7)
+//   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 17.0 (20.0)
+// 8-bit operands widened to 16 cost the tile kernels 1.9 times a k-tile (twice the products, and every wave
+// widens what it reads) and the thin one 1.08 times: 1.75 in relation.
+LinearChoice ChooseLinear(int kind, int out_type, int64_t rows, int k_tiles, int n_pad, bool copy, bool far_apart, int units) {
+  const double k = k_tiles, kt = kind == kMx8Exact ? 1.75 * k : k;
+  auto turns = [&](int r, int outputs) {
+    return std::ceil((double)((rows + r - 1) / r * ((n_pad + outputs - 1) / outputs)) / std::max(1, units));
+  };
+  auto thin_cost = [&](int r, int outputs, double on_16, double off) { return turns(r, outputs) * ((copy ? on_16 : off) * k + 0.5); };
+  const double thin[5] = {thin_cost(16, 16, 0.12, 0.18), thin_cost(16, 32, 0.19, 0.20), thin_cost(32, 16, 0.18, 0.33),
+                          thin_cost(32, 32, 0.25, 0.37), thin_cost(64, 32, 0.35, 0.66)};
+  const double t256 = turns(256, 256), t128 = turns(128, 128), t64 = turns(64, 64);
+  const double tile[7] = {t256 * (1.62 * kt + 7),
+                          t128 <= 1 ? 0.65 * kt + 2 : std::ceil(t128 / 2) * (0.95 * kt + 4),
+                          t128 * (0.55 * kt + 3),
+                          t64 <= 1 ? 0.31 * kt + 1 : std::ceil(t64 / 2) * (0.38 * kt + 2),
+                          t64 * (0.27 * kt + 1.5),
+                          t64 <= 1 ? 0.45 * kt : std::ceil(t64 / 4) * std::min(t64, 4.0) * 0.36 * kt,
+                          t128 <= 1 ? 1.25 * kt : std::ceil(t128 / 2) * 2.0 * kt};
+  // (with widened 8-bit operands the largest tile's registers do not suffice)
+  const int first = !copy ? 5 : kind == kMx8Exact ? 1 : 0, last = copy ? 5 : 7;
+  const int best = (int)(std::min_element(tile + first, tile + last) - tile);
+  // (a group of 32 8-bit outputs stays in one block)
+  int few = out_type == AMLIKE_MX8 ? 1 : 0;
+  for (int i = few + 1; i < 5; ++i)
+    if (thin[i] < thin[few] && (i != 2 || out_type != AMLIKE_MX8)) few = i;
+  if (thin[few] < tile[best] || far_apart) return {true, few};
+  return {false, best};
+}
 
 // ---- packing the weights ---------------------------------------------------------------------------------
 
@@ -73,6 +130,7 @@ using namespace amlike;
 struct amlike_linear {
   int device = 0;
   int k = 0, n = 0, n_pad = 0, k_tiles = 0, type = 0;
+  int max_blocks = kMaxBlocks;  // AMLIKE_LINEAR_MAX_BLOCKS: fewer, for tests of a call in several launches
   uint8_t *d_w = nullptr;
   uint32_t *d_scales = nullptr;
   float *d_bias = nullptr;
@@ -84,6 +142,11 @@ struct amlike_linear {
 
 namespace amlike {
 namespace {
+
+int PadOutputs(int n) { return (n + 63) / 64 * 64; }
+int KTiles(int k, int type) { return (int)(((int64_t)k * TypeBytes(type) + kTileBytes - 1) / kTileBytes); }
+// The kind of product of a layer's type for an output's.
+int KindOf(int type, int out_type) { return type == AMLIKE_MX8 && out_type == AMLIKE_F32 ? kMx8Exact : type; }
 
 int PackWeights(amlike_linear *h, const float *weights, int64_t ld, const float *bias) {
   const size_t row = (size_t)h->k * sizeof(float);
@@ -168,8 +231,9 @@ int amlike_linear_create(const float *weights, int32_t ld, const float *bias, in
   h->k = input_dim;
   h->n = output_dim;
   h->type = type;
-  h->n_pad = (output_dim + 63) / 64 * 64;
-  h->k_tiles = (int)(((int64_t)input_dim * TypeBytes(type) + kTileBytes - 1) / kTileBytes);
+  h->n_pad = PadOutputs(output_dim);
+  h->k_tiles = KTiles(input_dim, type);
+  if (const char *e = getenv("AMLIKE_LINEAR_MAX_BLOCKS")) h->max_blocks = std::max(1, std::min(kMaxBlocks, atoi(e)));
   const hipError_t e = hipStreamCreateWithFlags(&h->stream, hipStreamNonBlocking);
   int rc = AMLIKE_OK;
   if (e != hipSuccess) {
@@ -256,11 +320,35 @@ int amlike_linear_apply_dev(const amlike_linear_t *h, const amlike_matrix_t *x, 
   a.n_pad = h->n_pad;
   a.k_tiles = h->k_tiles;
   a.act = activation;
+  a.max_blocks = h->max_blocks;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (h->type == AMLIKE_BF16) return LaunchLinear<AMLIKE_BF16>(a, st);
-  if (h->type == AMLIKE_F16) return LaunchLinear<AMLIKE_F16>(a, st);
-  if (out->type == AMLIKE_F32) return LaunchLinear<kMx8Exact>(a, st);
+  const int kind = KindOf(h->type, out->type);
+  if (kind == AMLIKE_BF16) return LaunchLinear<AMLIKE_BF16>(a, st);
+  if (kind == AMLIKE_F16) return LaunchLinear<AMLIKE_F16>(a, st);
+  if (kind == kMx8Exact) return LaunchLinear<kMx8Exact>(a, st);
   return LaunchLinear<AMLIKE_MX8>(a, st);
+}
+
+const char *amlike_linear_kernel_info(int32_t type, int32_t out_type, int32_t rows, int32_t input_dim, int32_t output_dim,
+                                      int32_t aligned, int32_t units) {
+  static thread_local char text[128];
+  text[0] = 0;
+  if (type < AMLIKE_BF16 || type > AMLIKE_MX8 || out_type < AMLIKE_F32 || out_type > AMLIKE_MX8 || rows <= 0 || input_dim <= 0 ||
+      output_dim <= 0 || input_dim > kLinearMaxDim || output_dim > kLinearMaxDim || units <= 0 || units > 1 << 16)
+    return text;
+  const int kind = KindOf(type, out_type), n_pad = PadOutputs(output_dim);
+  const LinearChoice c = ChooseLinear(kind, out_type, rows, KTiles(input_dim, type), n_pad, aligned != 0, false, units);
+  if (c.thin) {
+    const ThinForm f = kThinForms[c.form];
+    snprintf(text, sizeof(text), "linear_thin_kernel<%d,%d,%d> rows=%d outputs=%d", kind, f.nt, f.mt, 16 * f.mt, 16 * f.nt);
+  } else {
+    const TileForm f = kTileForms[c.form];
+    const long long m = ((long long)rows + 16 * f.mf * f.wm - 1) / (16 * f.mf * f.wm), n = (n_pad + 64 * f.wn - 1) / (64 * f.wn);
+    snprintf(text, sizeof(text), "linear_pipe_kernel<%d,%d,%d,%d,%d,%d,%d> rows=%d outputs=%d tiles=%lld blocks=%lld", kind, f.wn, f.wm,
+             f.mf, f.stages, f.ks, f.copy ? 1 : 0, 16 * f.mf * f.wm, 64 * f.wn, m * n,
+             std::min<long long>((m * n + 7) & ~7LL, BlocksHeld(kind, f, units)));
+  }
+  return text;
 }
 
 int amlike_linear_apply(amlike_linear_t *h, const float *x, int32_t ld, int32_t rows, int32_t activation,

@@ -47,11 +47,39 @@ struct LinearArgs {
   int64_t ldx, ld_xs, ldr, ldo, ld_os;
   int32_t rows, k, n, n_pad, k_tiles;
   int32_t act, res_type, out_type;  // res_type -1: none
+  int32_t max_blocks;               // of a launch
 };
 
 // The kernels' kinds of product: a layer's type, or 8-bit operands with bf16 products.
 constexpr int kMx8Exact = 4;
 __host__ __device__ constexpr bool IsMx8(int kind) { return kind == AMLIKE_MX8 || kind == kMx8Exact; }
+
+// The forms of the tile kernel (linear_pipe_kernel's arguments) and of the kernel for few rows.
+struct TileForm {
+  int wn, wm, mf, stages, ks;
+  bool copy;
+};
+constexpr TileForm kTileForms[7] = {{4, 2, 8, 2, 1, true}, {2, 2, 4, 2, 1, true}, {2, 2, 4, 2, 2, true}, {1, 4, 1, 4, 1, true},
+                                    {1, 4, 1, 4, 2, true}, {1, 4, 1, 2, 1, false}, {2, 2, 4, 2, 1, false}};
+struct ThinForm {
+  int nt, mt;
+};
+constexpr ThinForm kThinForms[5] = {{1, 1}, {2, 1}, {1, 2}, {2, 2}, {2, 4}};
+
+// Waves a SIMD holds of a form, by its registers.
+constexpr int WavesPerSimd(int kind, const TileForm &f) { return !f.copy && f.mf == 1 && kind != kMx8Exact ? 4 : 2; }
+// As many blocks as the device holds at once, by waves and LDS, in eights.
+inline int BlocksHeld(int kind, const TileForm &f, int units) {
+  const int lds = f.ks * (64 * f.wn + 16 * f.mf * f.wm) * (f.stages * kTileBytes + (IsMx8(kind) ? 32 : 0)) + 64;
+  return std::max(8, (units * std::min(4 * WavesPerSimd(kind, f) / (f.wn * f.wm * f.ks), 163840 / lds)) & ~7);
+}
+// Which form a layer takes: of kThinForms if `thin`, else of kTileForms.  copy: 16-byte pieces of x can be copied as
+// they are; far_apart: its rows lie more than 4 MB apart.
+struct LinearChoice {
+  bool thin;
+  int form;
+};
+LinearChoice ChooseLinear(int kind, int out_type, int64_t rows, int k_tiles, int n_pad, bool copy, bool far_apart, int units);
 
 // The layer in one of the kinds, on `st`: defined for each kind in its own file.
 template <int KIND>
@@ -587,14 +615,10 @@ __device__ __forceinline__ uint32_t lds_address(T *p) {
 // Sixteen zero bytes: where pieces behind a row's end come from.
 static __device__ u32x4 g_zero_piece;
 
-// Waves a SIMD holds of a form, by its registers.
-template <int KIND, int MF, bool COPY>
-constexpr int kWavesPerSimd = !COPY && MF == 1 && KIND != kMx8Exact ? 4 : 2;
-
 // KS such groups of waves share a tile's k-tiles among them and add up at the end.  COPY: rows of x
 // start and end on 16 bytes; otherwise its pieces go through registers.
 template <int KIND, int WN, int WM, int MF, int STAGES, int KS, bool COPY>
-__global__ __launch_bounds__(64 * WN * WM * KS, (kWavesPerSimd<KIND, MF, COPY>)) void linear_pipe_kernel(LinearArgs a, int m_tiles, int n_tiles) {
+__global__ __launch_bounds__(64 * WN * WM * KS, (WavesPerSimd(KIND, TileForm{WN, WM, MF, STAGES, KS, COPY}))) void linear_pipe_kernel(LinearArgs a, int m_tiles, int n_tiles) {
   constexpr int kWaves = WN * WM, BN = 64 * WN, BM = 16 * MF * WM;
   constexpr bool kMx = IsMx8(KIND);
   static_assert(COPY || STAGES == 2, "one k-tile in registers");
@@ -1027,11 +1051,11 @@ __global__ __launch_bounds__(512) void linear_thin_kernel(LinearArgs a, int m_ti
 
 namespace {
 
-// Calls `launch` on stretches of the rows, all of them but for outputs beyond 2^22 blocks of `tile`
-// elements: a grid holds less than 2^32 threads, 2^23 blocks of 512.
+// Calls `launch` on stretches of the rows, all of them but for outputs beyond max_blocks (2^22) blocks of
+// `tile` elements: a grid holds less than 2^32 threads, 2^23 blocks of 512.
 template <typename F>
 int ByRows(LinearArgs a, int tile, F launch) {
-  const int64_t most = std::max<int64_t>(((int64_t)1 << 22) * tile / a.n_pad / 256 * 256, 256);
+  const int64_t most = std::max<int64_t>((int64_t)a.max_blocks * tile / a.n_pad / 256 * 256, 256);
   const int64_t rows = a.rows;
   const int rb = a.res_type < 0 ? 0 : TypeBytes(a.res_type), ob = TypeBytes(a.out_type);
   for (int64_t r = 0; r < rows; r += most) {
@@ -1046,15 +1070,14 @@ int ByRows(LinearArgs a, int tile, F launch) {
   return AMLIKE_OK;
 }
 
-template <int KIND, int WN, int WM, int MF, int STAGES, int KS, bool COPY = true>
+template <int KIND, int FORM>
 int LaunchPipe(const LinearArgs &args, hipStream_t st) {
   return ByRows(args, 2048, [&](const LinearArgs &a) -> int {
-    const int m_tiles = (a.rows + 16 * MF * WM - 1) / (16 * MF * WM), n_tiles = (a.n_pad + 64 * WN - 1) / (64 * WN);
-    // as many blocks as the device holds at once, by waves and LDS, in eights
-    constexpr int kLds = KS * (64 * WN + 16 * MF * WM) * (STAGES * kTileBytes + (IsMx8(KIND) ? 32 : 0)) + 64;
-    const int held = std::max(8, NumComputeUnits() * std::min(4 * kWavesPerSimd<KIND, MF, COPY> / (WN * WM * KS), 163840 / kLds) & ~7);
-    hipLaunchKernelGGL((linear_pipe_kernel<KIND, WN, WM, MF, STAGES, KS, COPY>), dim3((unsigned)std::min((m_tiles * n_tiles + 7) & ~7, held)),
-                       dim3(64 * WN * WM * KS), 0, st, a, m_tiles, n_tiles);
+    constexpr TileForm f = kTileForms[FORM];
+    const int m_tiles = (a.rows + 16 * f.mf * f.wm - 1) / (16 * f.mf * f.wm), n_tiles = (a.n_pad + 64 * f.wn - 1) / (64 * f.wn);
+    const int held = BlocksHeld(KIND, f, NumComputeUnits());
+    hipLaunchKernelGGL((linear_pipe_kernel<KIND, f.wn, f.wm, f.mf, f.stages, f.ks, f.copy>), dim3((unsigned)std::min((m_tiles * n_tiles + 7) & ~7, held)),
+                       dim3(64 * f.wn * f.wm * f.ks), 0, st, a, m_tiles, n_tiles);
     AMLIKE_HIP(hipGetLastError());
     return AMLIKE_OK;
   });
@@ -1067,8 +1090,9 @@ bool Copyable(const LinearArgs &a, int kind) {
          (!IsMx8(kind) || (reinterpret_cast<uintptr_t>(a.x_scales) | (uintptr_t)a.ld_xs) % 16 == 0);
 }
 
-template <int KIND, int NT, int MT>
+template <int KIND, int FORM>
 int LaunchThin(const LinearArgs &args, hipStream_t st) {
+  constexpr int NT = kThinForms[FORM].nt, MT = kThinForms[FORM].mt;
   return ByRows(args, 256 * NT * MT, [&](const LinearArgs &a) -> int {
     const int m_tiles = (a.rows + 16 * MT - 1) / (16 * MT), n_tiles = a.n_pad / (16 * NT);
     const unsigned blocks = (unsigned)((std::max(m_tiles, n_tiles) + 7) & ~7) * std::min(m_tiles, n_tiles);
@@ -1078,73 +1102,27 @@ int LaunchThin(const LinearArgs &args, hipStream_t st) {
   });
 }
 
-// The form with the least estimated time, from the turns that the busiest compute unit has to take.
-// Microseconds per k-tile and per turn, measured in bf16 at the sizes behind each line (less the
-// 2.2 that every launch takes); only their relation matters.
-//   256 x 256, 8 waves                      1.62 kt + 7    35554 x 2000 x 8600: 1118 (measured 1157)
-//   128 x 128, 4 waves, alone on its unit   0.65 kt + 2    1024 x 4096 x 4096: 44 (44.5)
-//              two of them                  0.95 kt + 4    4096 x 2048 x 2048: 34 (34.4)
-//   128 x 128, 2 groups of 4 waves          0.55 kt + 3    1024 x 4096 x 4096: 38 (38.7)
-//   64 x 64, 4 waves, alone                 0.31 kt + 1    300 x 360 x 2000: 2.9 (5.5 with the launch)
-//            two of them                    0.38 kt + 2    1024 x 4096 x 4096: 53 (54)
-//   64 x 64, 2 groups of 4 waves            0.27 kt + 1.5  32 x 4096 x 16384: 21 (22.4 with it)
-// Rows of x that do not start and end on 16 bytes go through registers, in two forms:
-//   64 x 64, four blocks a unit             0.36 kt each   1237 x 1999 x 2001 bf16: 30.0 (128 x 128: 39.5)
-//            alone                          0.45 kt        64 x 2000 x 1024: 14.4 (16.0 with it)
-//   128 x 128, alone / two of them   1.25 kt / 2.0 kt      2000 x 2002 x 4096 mx8: 32.0 (64 x 64: 53.1)
-// The thin kernel, whatever the rows' places; the second figure where they are not on 16 bytes
-// (sizes and times as above, all with the launch), and 0.5 a turn:
-//   16 rows x 16 outputs                    0.12, 0.18 kt  64 x 4096 x 1024: 9.5 (64 x 64: 21.3)
-//   16 rows x 32 outputs                    0.19, 0.20 kt  16 x 8192 x 8192: 24.9 (16 x 16: 31.1)
-//   32 rows x 16 outputs                    0.18, 0.33 kt  128 x 4096 x 1024: 13.0 (64 x 64: 21.4)
-//   32 rows x 32 outputs                    0.25, 0.37 kt  64 x 4096 x 4096: 17.5 (64 x 64: 21.7)
-//   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 17.0 (20.0)
-// 8-bit operands widened to 16 cost the tile kernels 1.9 times a k-tile (twice the products, and every wave
-// widens what it reads) and the thin one 1.08 times: 1.75 in relation.
 }  // namespace
 
 template <int KIND>
 int LaunchLinear(const LinearArgs &a, hipStream_t st) {
-  const double units = std::max(1, NumComputeUnits()), k_tiles = a.k_tiles, kt = KIND == kMx8Exact ? 1.75 * k_tiles : k_tiles;
-  auto turns = [&](int rows, int outputs) {
-    return std::ceil((double)(((int64_t)a.rows + rows - 1) / rows * ((a.n_pad + outputs - 1) / outputs)) / units);
-  };
-  const bool copy = Copyable(a, KIND);
-  auto thin_cost = [&](int rows, int outputs, double on_16, double off) {
-    return turns(rows, outputs) * ((copy ? on_16 : off) * k_tiles + 0.5);
-  };
-  const double thin[5] = {thin_cost(16, 16, 0.12, 0.18), thin_cost(16, 32, 0.19, 0.20), thin_cost(32, 16, 0.18, 0.33),
-                          thin_cost(32, 32, 0.25, 0.37), thin_cost(64, 32, 0.35, 0.66)};
-  const double t256 = turns(256, 256), t128 = turns(128, 128), t64 = turns(64, 64);
-  double tile[7] = {t256 * (1.62 * kt + 7),
-                    t128 <= 1 ? 0.65 * kt + 2 : std::ceil(t128 / 2) * (0.95 * kt + 4),
-                    t128 * (0.55 * kt + 3),
-                    t64 <= 1 ? 0.31 * kt + 1 : std::ceil(t64 / 2) * (0.38 * kt + 2),
-                    t64 * (0.27 * kt + 1.5),
-                    t64 <= 1 ? 0.45 * kt : std::ceil(t64 / 4) * std::min(t64, 4.0) * 0.36 * kt,
-                    t128 <= 1 ? 1.25 * kt : std::ceil(t128 / 2) * 2.0 * kt};
-  // (with widened 8-bit operands the largest tile's registers do not suffice)
-  const int first = !copy ? 5 : KIND == kMx8Exact ? 1 : 0, last = copy ? 5 : 7;
-  const int best = (int)(std::min_element(tile + first, tile + last) - tile);
-  // (a group of 32 8-bit outputs stays in one block)
-  int few = a.out_type == AMLIKE_MX8 ? 1 : 0;
-  for (int i = few + 1; i < 5; ++i)
-    if (thin[i] < thin[few] && (i != 2 || a.out_type != AMLIKE_MX8)) few = i;
   // (the tile kernel addresses a tile's rows with 32 bits)
-  if (thin[few] < tile[best] || a.ldx > 1 << 22 || a.ld_xs > 1 << 22) {
-    if (few == 0) return LaunchThin<KIND, 1, 1>(a, st);
-    if (few == 1) return LaunchThin<KIND, 2, 1>(a, st);
-    if (few == 2) return LaunchThin<KIND, 1, 2>(a, st);
-    if (few == 3) return LaunchThin<KIND, 2, 2>(a, st);
-    return LaunchThin<KIND, 2, 4>(a, st);
+  const bool far_apart = a.ldx > 1 << 22 || a.ld_xs > 1 << 22;
+  const LinearChoice c = ChooseLinear(KIND, a.out_type, a.rows, a.k_tiles, a.n_pad, Copyable(a, KIND), far_apart, NumComputeUnits());
+  if (c.thin) {
+    if (c.form == 0) return LaunchThin<KIND, 0>(a, st);
+    if (c.form == 1) return LaunchThin<KIND, 1>(a, st);
+    if (c.form == 2) return LaunchThin<KIND, 2>(a, st);
+    if (c.form == 3) return LaunchThin<KIND, 3>(a, st);
+    return LaunchThin<KIND, 4>(a, st);
   }
-  if (best == 1) return LaunchPipe<KIND, 2, 2, 4, 2, 1>(a, st);
-  if (best == 2) return LaunchPipe<KIND, 2, 2, 4, 2, 2>(a, st);
-  if (best == 3) return LaunchPipe<KIND, 1, 4, 1, 4, 1>(a, st);
-  if (best == 4) return LaunchPipe<KIND, 1, 4, 1, 4, 2>(a, st);
-  if (best == 5) return LaunchPipe<KIND, 1, 4, 1, 2, 1, false>(a, st);
-  if (best == 6) return LaunchPipe<KIND, 2, 2, 4, 2, 1, false>(a, st);
-  if constexpr (KIND != kMx8Exact) return LaunchPipe<KIND, 4, 2, 8, 2, 1>(a, st);
+  if (c.form == 1) return LaunchPipe<KIND, 1>(a, st);
+  if (c.form == 2) return LaunchPipe<KIND, 2>(a, st);
+  if (c.form == 3) return LaunchPipe<KIND, 3>(a, st);
+  if (c.form == 4) return LaunchPipe<KIND, 4>(a, st);
+  if (c.form == 5) return LaunchPipe<KIND, 5>(a, st);
+  if (c.form == 6) return LaunchPipe<KIND, 6>(a, st);
+  if constexpr (KIND != kMx8Exact) return LaunchPipe<KIND, 0>(a, st);
   return AMLIKE_EINVAL;
 }
 

@@ -113,6 +113,12 @@ class RmsNorm:
             _lib.check(rc)
 
 
+def linear_kernel_info(type, out, rows, input_dim, output_dim, aligned=True, units=256):
+    """The kernel and form that Linear.ApplyDevice takes (amlike_linear_kernel_info); needs no GPU."""
+    args = [_int32(v, "size") for v in (rows, input_dim, output_dim)]
+    return _lib.lib().amlike_linear_kernel_info(TYPES[type], TYPES[out], *args, int(aligned), _int32(units, "units")).decode()
+
+
 class Linear:
     """out = act(x weights^T + bias) + residual; weights [output x input], in `type` ("bf16", "f16", "mx8")."""
 
