@@ -326,10 +326,12 @@ int32_t amlike_linear_device(const amlike_linear_t *linear);
  * or F16, or NULL) and out (any type) are [rows x output_dim].  rows may be 0.  out may be the
  * same matrix as residual (same data, type and ld); no other overlap is allowed.  A row's result
  * does not depend on the other rows' values.  MX8 layers: for an F32 output the products are
- * summed as exactly as those of the other types, whatever the scales (scale bytes of x from 244 up, values beyond
- * 1e35 that is, and groups of weights below 1e-34 that are not 0, take ten times as long for the
- * rows and outputs around them); for the smaller outputs by the 8-bit matrix instruction, whose sums
- * are about 1.5e-5 off, relative to the sum of normal values, and twice as fast. */
+ * summed as exactly as those of the other types, whatever the scales (scale bytes of x from 244 up, groups with a
+ * value beyond 3.7e37 that is, and groups of weights all below 8e-35 but not 0, take ten to twenty times as long
+ * for the rows and outputs around them); for the smaller outputs by the 8-bit matrix instruction, which
+ * is twice as fast and whose sums are about 1.5e-5 off, relative to the sum of normal values (where a
+ * sum cancels, to its summands).  Activations are a few units of fp32 off; gelu for outputs smaller than F32
+ * 3.5e-5, relative to the normal distribution's tail beyond |x|.  Results below fp32's normal range may be 0. */
 int amlike_linear_apply_dev(const amlike_linear_t *linear, const amlike_matrix_t *x, int32_t rows,
                             int32_t activation, const amlike_matrix_t *residual,
                             const amlike_matrix_t *out, void *stream);

@@ -22,8 +22,8 @@ extern template int LaunchLinear<kMx8Exact>(const LinearArgs &, hipStream_t);
 // ---- the choice of a form ---------------------------------------------------------------------------------
 
 // The form with the least estimated time, from the turns that the busiest compute unit has to take.
-// Microseconds per k-tile and per turn, measured in bf16 at the sizes behind each line (less the
-// 2.2 that every launch takes); only their relation matters.
+// Microseconds per k-tile and per turn, measured in bf16 at the sizes behind each line with W in the caches (less
+// the 2.2 that every launch takes); only their relation matters.
 //   256 x 256, 8 waves                      1.62 kt + 7    35554 x 2000 x 8600: 1118 (measured 1157)
 //   128 x 128, 4 waves, alone on its unit   0.65 kt + 2    1024 x 4096 x 4096: 44 (44.5)
 //              two of them                  0.95 kt + 4    4096 x 2048 x 2048: 34 (34.4)
@@ -41,7 +41,7 @@ extern template int LaunchLinear<kMx8Exact>(const LinearArgs &, hipStream_t);
 //   16 rows x 32 outputs                    0.19, 0.20 kt  16 x 8192 x 8192: 24.9 (16 x 16: 31.1)
 //   32 rows x 16 outputs                    0.18, 0.33 kt  128 x 4096 x 1024: 13.0 (64 x 64: 21.4)
 //   32 rows x 32 outputs                    0.25, 0.37 kt  64 x 4096 x 4096: 17.5 (64 x 64: 21.7)
-//   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 17.0 (20.0)
+//   64 rows x 32 outputs                    0.35, 0.66 kt  256 x 4096 x 2048 mx8 to f32: 17.2 (20.0)
 // 8-bit operands widened to 16 cost the tile kernels 1.9 times a k-tile (twice the products, and every wave
 // widens what it reads) and the thin one 1.08 times: 1.75 in relation.
 LinearChoice ChooseLinear(int kind, int out_type, int64_t rows, int k_tiles, int n_pad, bool copy, bool far_apart, int units) {

@@ -12,8 +12,8 @@
 // The 8-bit instruction aligns the products of a few neighbouring columns to the largest of them
 // and drops what lies more than 13 binary places below it (measured: 2^16 + 2^2 is 2^16, 2^16 + 2^3
 // is whole), which leaves a relative error of about 1.5e-5 in a sum of normal values whatever its
-// length: far below the rounding of a 16-bit (2^-9, 2^-12 on average) or 8-bit output, too much for
-// an fp32 one.  For an fp32 output the 8-bit operands are therefore widened to bf16, which holds
+// length: below a hundredth of the rounding of a bf16 (up to 2^-8) or 8-bit output (2^-4) and a thirtieth of an f16
+// one's (2^-11), too much for an fp32 one.  (Where a sum cancels, it is relative to the summands, not to the result.)  For an fp32 output the 8-bit operands are therefore widened to bf16, which holds
 // value times scale exactly but for scales at the ends of their range (is_far_x), and multiplied there
 // (kMx8Exact), at half the matrix rate.  A wave that met such a scale takes its sums once more, group
 // by group (far_sums).
@@ -721,7 +721,7 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (WavesPerSimd(KIND, TileForm{WN,
         const int64_t line = (int64_t)(kt >> 2) * a.n_pad + (n0 + r < a.n_pad ? n0 + r : 0);
         const uint8_t *base = of_w ? reinterpret_cast<const uint8_t *>(a.w_scales) + line * 16 : a.x_scales + m0 * a.ld_xs + (int64_t)kt * 4;
         const uint32_t offset = of_w ? row_at_place(lane) * 16 : (uint32_t)min(r - BN + lane, last_row()) * (uint32_t)a.ld_xs;
-        if constexpr (COPY) {  // (what a row's last 16 bytes hold behind its last scale is put right on reading)
+        if constexpr (COPY) {  // (what a row's last 16 bytes hold behind its last scale is put right on reading; being aligned, they leave no page)
           copy16_to_lds(base, offset, lds_address(&s_scales[ks][step >> 2 & 1][r]));
         } else {
           typedef u32x4 u32x4_byte __attribute__((aligned(1)));
@@ -900,8 +900,9 @@ __global__ __launch_bounds__(64 * WN * WM * KS, (WavesPerSimd(KIND, TileForm{WN,
 // ---- few rows ------------------------------------------------------------------------------------------
 // 16 NT outputs x 16 MT rows per block; its eight waves share the k-tiles among them, each from
 // memory straight into registers, and add up in LDS in wave order; kBatch k-tiles of each are in
-// flight.  For few rows the way of W from HBM bounds it (16 x 8192 x 8192 bf16: 24.9 us, 5.4 TB/s), for
-// small products a launch and two trips to memory (1 x 2048 x 2048 bf16: 4.6 us, of which 2.2 are any
+// flight.  For few rows the way of W bounds it (16 x 8192 x 8192 bf16: 26.2 us and 5.1 TB/s from HBM, six layers of
+// 134 MB in turn; 25.2 us with the one layer's W in the last-level cache), for small products a launch and two
+// trips to memory (1 x 2048 x 2048 bf16: 6.3 us from HBM, 80 layers in turn, 4.7 from the caches, of which 2.2 are any
 // launch's).  (Tried: biases and residual asked for before the k-tiles, 0; the k-tile that rows end in
 // moved out of the batches, 0; eight whole lines a load instead of sixteen halves, with lanes trading
 // pieces, -5 %.)
