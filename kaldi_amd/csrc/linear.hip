@@ -1,5 +1,5 @@
-// amlike_linear_*: the host side of the matrix product with bias, activation and residual, and the
-// packing of its weights.  The kernels: linear_kernels.h.
+// amlike_linear_*: the host side of the matrix product with bias, activation and residual, the choice of
+// a kernel's form, and the packing of the weights.  The kernels: linear_kernels.h.
 #include <algorithm>
 #include <cmath>
 #include <cstdio>

@@ -12,17 +12,18 @@
 // The 8-bit instruction aligns the products of a few neighbouring columns to the largest of them
 // and drops what lies more than 13 binary places below it (measured: 2^16 + 2^2 is 2^16, 2^16 + 2^3
 // is whole), which leaves a relative error of about 1.5e-5 in a sum of normal values whatever its
-// length: below a hundredth of the rounding of a bf16 (up to 2^-8) or 8-bit output (2^-4) and a thirtieth of an f16
-// one's (2^-11), too much for an fp32 one.  (Where a sum cancels, it is relative to the summands, not to the result.)  For an fp32 output the 8-bit operands are therefore widened to bf16, which holds
-// value times scale exactly but for scales at the ends of their range (is_far_x), and multiplied there
-// (kMx8Exact), at half the matrix rate.  A wave that met such a scale takes its sums once more, group
-// by group (far_sums).
+// length (where a sum cancels, relative to the summands): below a hundredth of the rounding of a bf16
+// (up to 2^-8) or 8-bit output (2^-4), a thirtieth of an f16 one's (2^-11), too much for an fp32 one.
+// For an fp32 output the 8-bit operands are therefore widened to bf16, which holds value times scale
+// exactly but for scales at the ends of their range (is_far_x), and multiplied there (kMx8Exact), at
+// half the matrix rate.  A wave that met such a scale takes its sums once more, group by group
+// (far_sums).
 //   W:      [k-tile][row, padded to 64][128 bytes], zeros behind both ends
 //   scales: [k-tile / 4][row, padded to 64][k-tile % 4][4 bytes], 2^0 behind both ends and for groups
 //           of zeros  (8 bits only)
 //
-// This header holds the kernels and the choice between them; each kind of product is compiled in a file
-// of its own (linear_bf16.hip ...), the host side is linear.hip.
+// This header holds the kernels and their launches; each kind of product is compiled in a file of its
+// own (linear_bf16.hip ...), the choice of a form and the host side are in linear.hip.
 #ifndef KALDI_AMD_CSRC_LINEAR_KERNELS_H_
 #define KALDI_AMD_CSRC_LINEAR_KERNELS_H_
 

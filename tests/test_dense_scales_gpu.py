@@ -141,3 +141,31 @@ def test_far_scales_of_one_column_and_of_short_rows(amlike_device):
             lin.ApplyDevice(m.m, 5, out.m)
             torch.cuda.synchronize()
             assert torch.equal(out.values(), want) and math.isfinite(float(want.max()))
+
+
+@pytest.mark.parametrize("rows,k,n,pad", [(1000, 208, 130, 16), (700, 333, 70, 3), (600, 1040, 2000, 16)])
+def test_far_scales_in_a_call_of_several_launches(amlike_device, monkeypatch, rows, k, n, pad):
+    """Each launch finds the scales of its own rows; replayed from a graph it gives the same."""
+    monkeypatch.setenv("AMLIKE_LINEAR_MAX_BLOCKS", "1")
+    groups = (k + 31) // 32
+    of = torch.full((rows, groups), 127)
+    of[::101, ::3] = 254
+    of[50::77] = 0
+    xi, wi = ints(rows, k, -8, 8, 7), ints(n, k, -8, 8, 8)
+    lin = dense.Linear(wi.numpy(), None, "mx8")
+    x = matrix(codes(xi * 2.0 ** -9), of, pad)
+    want = (xi * torch.exp2(of.double() - 136).repeat_interleave(32, dim=1)[:, :k]) @ wi.t()
+    same = (of == of[:, :1]).all(1)  # (rows of one scale: their sums are exact)
+    got = apply(lin, x, n, "f32", pad)
+    assert same.sum() > rows // 2 and torch.equal(got[same], want[same])
+    mass = (xi.abs() * torch.exp2(of.double() - 136).repeat_interleave(32, dim=1)[:, :k]) @ wi.abs().t()
+    over = torch.isinf(got) & (mass >= 2.0 ** 127)  # (no partial sum passes the mass; one beyond fp32's range is infinite)
+    assert (over | ((got - want).abs() <= (k + 1) * 2.0 ** -23 * mass)).all() and not over[::101].all()
+    out, graph, stream = U.DeviceMatrix(rows, n, "f32"), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        lin.ApplyDevice(x.m, rows, out.m, stream=stream.cuda_stream)
+    for _ in range(3):
+        out.buf.fill_(0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.values(), got)
